@@ -59,6 +59,16 @@ class HxqDecoderLayer(ctypes.Structure):
     ]
 
 
+class HxqKv8(ctypes.Structure):
+    """Mirror of ``hxq_kv8`` in include/hxq.h."""
+
+    _fields_ = [
+        ("k", P), ("v", P), ("k_scale", P), ("v_scale", P), ("k_tail", P), ("v_tail", P),
+        ("blocks", P), ("dtype", I32), ("batch", I32), ("n_kv_heads", I32), ("head_dim", I32),
+        ("n_blocks", I32),
+    ]
+
+
 class HxqDecoder(ctypes.Structure):
     """Mirror of ``hxq_decoder`` in include/hxq.h (``layers`` is a host array)."""
 
@@ -103,6 +113,13 @@ SIGNATURES = {
     "hxq_attn_rope_decode": [P, P, I32, I32, I32, F32, P, P, I32, I32, P, I32, P],
     "hxq_dense_gemv_bf16": [P, P, I32, I64, I64, P, P],
     "hxq_argmax": [P, I64, P, P, P, P],
+    "hxq_attn_prompt": [P, I64, I64, P, I64, I64, P, I64, I64, I32, P, P, I32, I64, I64, I32, I32,
+                        I32, F32, I32, P, I64, I64, P],
+    "hxq_kv8_append": [P, I64, I64, P, I64, I64, P, I64, I64, I32, P, I64, I32, P, P, F32, P, P, P,
+                       P, P],
+    "hxq_kv8_attn_decode": [P, I64, I64, P, I64, I64, P, I64, I64, I32, I32, P, P, F32, F32, P, P,
+                            P, P, I32, P, I64, P],
+    "hxq_kv8_evict": [P, P, P, I32, I32, I32, I32, I32, I32, P, P, P, P],
     "hxq_moe_grouped_tile": [I64, I32, I32, I64, I32],
     "hxq_moe_grouped_gemm": [P, I32, I64, P, P, I64, I32, P, I32, P, I32, I64, I64, P],
     "hxq_moe_ffn": [P, I32, I64, I64, I64, I32, I32, P, P, P, P, P, P, P, I32, P, I64, P, I32, P],
@@ -138,6 +155,7 @@ SIGNATURES_I64 = {
     "hxq_gemm_workspace_bytes": [I64, I64, I64],
     "hxq_gemm_noalloc_max_bytes": [],
     "hxq_prefill_gemm_workspace_bytes": [I64, I64, I64],
+    "hxq_kv8_attn_decode_workspace_bytes": [I32, I32, I32, I32, I32, I32],
     "hxq_prefill_gemm_plan": [I64, I64, I64, I32, I32, I32],
 }
 
@@ -147,7 +165,7 @@ def library_path() -> Path:
 
 
 # HXQ_ABI_VERSION of include/hxq.h that the ctypes signatures below follow
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 
 def lib():
@@ -788,6 +806,167 @@ def attn_rope_decode(qkv, pos, n_heads, n_kv, head_dim, theta, k_cache, v_cache,
                                     _stream(qkv))
     _check("hxq_attn_rope_decode", rc)
     return out
+
+
+# -- attention of prompts and the 8-bit KV cache ---------------------------------
+KV8_BLOCK = 64
+
+
+def _need_heads_of(**named):
+    """q, k, v, out: [rows, heads, head_dim] views on one device, head_dim contiguous (any row and
+    head stride that the library takes); returns the device."""
+    dev = index = None
+    for name, t in named.items():
+        if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+            raise ValueError(f"{name} must be [rows, heads, head_dim] with head_dim contiguous")
+        i = t.get_device()
+        if i < 0 or not t.is_cuda:
+            raise RuntimeError("HXQ kernels take device tensors only")
+        if dev is None:
+            dev, index = t.device, i
+        elif i != index:
+            raise RuntimeError(f"tensors on different devices: {dev} vs {t.device}")
+    return dev
+
+
+def _view(t):
+    """Pointer, row stride and head stride; strides that no element needs count as 0."""
+    r, h, _ = t.shape
+    return t.data_ptr(), t.stride(0) if r > 1 else 0, t.stride(1) if h > 1 else 0
+
+
+def _on(t):
+    """The current device for the call when it is not the tensor's (the library asks it for its
+    compute units)."""
+    return torch.cuda.device(t.device) if torch.cuda.current_device() != t.get_device() else None
+
+
+def _kv8_call(t, name, *args):
+    fn, dev = getattr(lib(), name), _on(t)
+    if dev is None:
+        _check(name, fn(*args))
+    else:
+        with dev:
+            _check(name, fn(*args))
+
+
+def attn_prompt(q, k, v, cu_q, cu_k, scale, causal, out):
+    """Attention of packed prompts (hxq_attn_prompt): q [rows, heads, D], k and v [rows, kv heads,
+    D], bf16 or fp16, cu_* int32 [n_seqs + 1]; out as q."""
+    dev = _need_heads_of(q=q, k=k, v=v, out=out)
+    if not q.dtype == k.dtype == v.dtype == out.dtype:
+        raise RuntimeError(f"q, k, v and out must have one dtype (got {q.dtype}, {k.dtype}, "
+                           f"{v.dtype}, {out.dtype})")
+    if k.shape != v.shape or k.shape[2] != q.shape[2] or out.shape != q.shape:
+        raise ValueError("shapes must be q, out [rows, heads, D], k, v [rows, kv heads, D]")
+    _need_i32(cu_q=cu_q, cu_k=cu_k)
+    if _need_device(cu_q, cu_k) != dev:
+        raise RuntimeError("tensors on different devices")
+    if cu_q.dim() != 1 or cu_q.numel() < 1 or (cu_k is not None and cu_k.shape != cu_q.shape):
+        raise ValueError("cu_q and cu_k must be [n_seqs + 1]")
+    if cu_k is None and k.shape[0] != q.shape[0]:
+        raise ValueError("k needs as many rows as q, or cu_k")
+    _kv8_call(q, "hxq_attn_prompt", *_view(q), *_view(k), *_view(v), dtype_code(q.dtype), _ptr(cu_q),
+              _ptr(cu_k), cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1],
+              q.shape[2], float(scale), int(causal), *_view(out), _stream(q))
+    return out
+
+
+def kv8_desc(k, v, k_scale, v_scale, k_tail, v_tail, blocks):
+    """hxq_kv8 of a cache's tensors."""
+    _need_device(k, v, k_scale, v_scale, k_tail, v_tail, blocks)
+    batch, n_kv, n_blocks, block, D = k.shape
+    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
+        raise RuntimeError("k and v must be float8_e4m3fn")
+    if k_tail.dtype not in (torch.bfloat16, torch.float16) or v_tail.dtype != k_tail.dtype:
+        raise RuntimeError("k_tail and v_tail must be bfloat16 or float16, both alike")
+    _need_f32(k_scale=k_scale, v_scale=v_scale)
+    _need_i32(blocks=blocks)
+    each = (batch, n_kv, n_blocks)
+    if (block != KV8_BLOCK or v.shape != (*each, D, block) or k_scale.shape != each
+            or v_scale.shape != each or k_tail.shape != (batch, n_kv, block, D)
+            or v_tail.shape != (batch, n_kv, D, block)
+            or (blocks is not None and blocks.shape != each)):
+        raise ValueError("cache shapes do not fit together")
+    return HxqKv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                  k_tail.data_ptr(), v_tail.data_ptr(), _ptr(blocks), dtype_code(k_tail.dtype),
+                  batch, n_kv, D, n_blocks)
+
+
+def kv8_append(q, k, v, cu_rows, cached, pos, theta, desc, q_out, k_out, v_out):
+    """Rows of packed prompts into the cache (hxq_kv8_append).  q may be None with q_out None."""
+    dev = _need_heads_of(k=k, v=v) if q is None else _need_heads_of(q=q, k=k, v=v)
+    _need_i32(cu_rows=cu_rows, cached=cached, pos=pos)
+    if _need_device(cu_rows, cached, pos, q_out, k_out, v_out) != dev:
+        raise RuntimeError("tensors on different devices")
+    rows, n_kv, D = k.shape
+    if (v.shape != k.shape or n_kv != desc.n_kv_heads or D != desc.head_dim
+            or (q is not None and (q.shape[0] != rows or q.shape[2] != D))):
+        raise ValueError("q must be [rows, heads, D], k and v [rows, kv heads, D] of the cache")
+    if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype):
+        raise RuntimeError("q, k and v must have one dtype")
+    if cu_rows.shape != (desc.batch + 1,) or cached.shape != (desc.batch,) or (
+            pos is not None and pos.shape != (desc.batch,)):
+        raise ValueError("cu_rows must be [batch + 1], cached and pos [batch]")
+    for t, like in ((q_out, q), (k_out, k), (v_out, v)):
+        if t is not None and (like is None or t.shape != like.shape
+                              or dtype_code(t.dtype) != desc.dtype):
+            raise ValueError("outputs must have the rows' shapes and the cache's 16-bit dtype")
+    heads = n_kv if q is None else q.shape[1]
+    _kv8_call(k, "hxq_kv8_append", *((None, 0, 0) if q is None else _view(q)), *_view(k), *_view(v),
+              dtype_code(k.dtype), _ptr(cu_rows), rows, heads, _ptr(cached), _ptr(pos),
+              float(theta), ctypes.byref(desc), _ptr(q_out), _ptr(k_out), _ptr(v_out), _stream(k))
+
+
+def kv8_attn_decode(q, k, v, cached, pos, theta, scale, desc, weight, weight_out, out):
+    """One token of each sequence over its cache (hxq_kv8_attn_decode)."""
+    dev = _need_heads_of(q=q, k=k, v=v)
+    _need_i32(cached=cached, pos=pos)
+    _need_f32(weight=weight, weight_out=weight_out)
+    if _need_device(cached, pos, weight, weight_out, out) != dev:
+        raise RuntimeError("tensors on different devices")
+    batch, heads, D = q.shape
+    if (batch != desc.batch or D != desc.head_dim or v.shape != k.shape
+            or k.shape != (batch, desc.n_kv_heads, D) or out.shape != q.shape):
+        raise ValueError("q and out must be [batch, heads, D], k and v [batch, kv heads, D] of the "
+                         "cache")
+    if not q.dtype == k.dtype == v.dtype:
+        raise RuntimeError("q, k and v must have one dtype")
+    if cached.shape != (batch,) or (pos is not None and pos.shape != (batch,)):
+        raise ValueError("cached and pos must be [batch]")
+    each = (batch, desc.n_kv_heads, desc.n_blocks)
+    for t in (weight, weight_out):
+        if t is not None and t.shape != each:
+            raise ValueError("weights must be [batch, kv heads, n_blocks]")
+    nbytes = _kv8_workspace(batch, heads, desc.n_kv_heads, D, desc.n_blocks, weight_out is not None,
+                            q.get_device())
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
+    _kv8_call(q, "hxq_kv8_attn_decode", *_view(q), *_view(k), *_view(v), dtype_code(q.dtype), heads,
+              _ptr(cached), _ptr(pos), float(theta), float(scale), ctypes.byref(desc), _ptr(weight),
+              _ptr(weight_out), _ptr(out), dtype_code(out.dtype), _ptr(ws), nbytes, _stream(q))
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _kv8_workspace(batch, heads, n_kv, D, n_blocks, weights, device):
+    """hxq_kv8_attn_decode_workspace_bytes on `device` (it counts the compute units)."""
+    with torch.cuda.device(device):
+        return lib().hxq_kv8_attn_decode_workspace_bytes(batch, heads, n_kv, D, n_blocks, int(weights))
+
+
+def kv8_evict(weight, blocks, cached, keep, sink, recent, weight_out, blocks_out, cached_out):
+    """Choose the blocks that stay (hxq_kv8_evict)."""
+    _need_device(weight, blocks, cached, weight_out, blocks_out, cached_out)
+    _need_f32(weight=weight, weight_out=weight_out)
+    _need_i32(blocks=blocks, cached=cached, blocks_out=blocks_out, cached_out=cached_out)
+    if weight.dim() != 3 or cached.shape != weight.shape[:1] or any(
+            t is not None and t.shape != weight.shape for t in (blocks, weight_out, blocks_out)
+    ) or cached_out.shape != cached.shape:
+        raise ValueError("weights and blocks must be [batch, kv heads, n_blocks], cached [batch]")
+    batch, n_kv, n_blocks = weight.shape
+    _kv8_call(weight, "hxq_kv8_evict", _ptr(weight), _ptr(blocks), _ptr(cached), batch, n_kv,
+              n_blocks, int(keep), int(sink), int(recent), _ptr(weight_out), _ptr(blocks_out),
+              _ptr(cached_out), _stream(weight))
 
 
 def silu_mul(gate, up, out):

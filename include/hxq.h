@@ -102,8 +102,10 @@ const char *hxq_last_error(void);
  *   3: wide scalar encoder entry points (hxq_assign_nearest_wide,
  *      hxq_kmeans_run_wide, hxq_affine_fit_wide); hxq_kmeans_workspace_bytes
  *      sizes for codebooks of up to 4096 entries.
+ *   4: attention over prompts and the 8-bit KV cache (hxq_attn_prompt,
+ *      hxq_kv8_append, hxq_kv8_attn_decode, hxq_kv8_evict).
  */
-#define HXQ_ABI_VERSION 3
+#define HXQ_ABI_VERSION 4
 int hxq_abi_version(void);
 
 /*
@@ -522,6 +524,118 @@ int hxq_dense_gemv_bf16(const uint16_t *weight, const void *x, int32_t x_dtype, 
                         int64_t in_features, float *y, hipStream_t stream);
 int hxq_argmax(const float *logits, int64_t n, int32_t *out_id, int32_t *pos,
                void *workspace, hipStream_t stream);
+
+/*
+ * Attention over prompts, and a KV cache held in 8 bits.  No reference counterparts (the
+ * reference leaves attention and the cache to transformers' Qwen2, models/qwen2/modeling_qwen2.py).
+ * Unlike the rest of this header these entry points take q, k and v as views
+ * [rows, heads, head_dim] with a row and a head stride in elements (head_dim contiguous; pointers
+ * and strides multiples of 16 bytes), so that slices of a fused projection need no copy.
+ * Query head h reads kv head h / (n_heads / n_kv_heads); head_dim is 64 or 128.
+ */
+
+/*
+ * Attention of packed prompts.  Sequence s owns the query rows cu_q[s] .. cu_q[s + 1] and the key
+ * rows cu_k[s] .. cu_k[s + 1] (device int32 [n_seqs + 1]; cu_k NULL = cu_q):
+ *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j]) v[j]
+ * over the sequence's keys j; causal: j <= i + (keys - queries), both counted in the sequence, so a
+ * prompt that continues cached tokens passes them as its first keys.  A query that sees no key
+ * gives zeros.  Keys that a query does not see have no influence, whatever they hold.  dtype (q, k,
+ * v, out): HXQ_BF16 or HXQ_F16; scores, softmax and sums are fp32, the softmax weights are rounded
+ * to dtype before the product with v.  Rows of out that belong to no sequence are left as they
+ * were; offsets are clamped to [0, rows_q] and [0, rows_k].
+ */
+int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
+                    int64_t k_row_stride, int64_t k_head_stride, const void *v,
+                    int64_t v_row_stride, int64_t v_head_stride, int32_t dtype,
+                    const int32_t *cu_q, const int32_t *cu_k, int32_t n_seqs, int64_t rows_q,
+                    int64_t rows_k, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                    float scale, int32_t causal, void *out, int64_t out_row_stride,
+                    int64_t out_head_stride, hipStream_t stream);
+
+/*
+ * The 8-bit cache: per sequence and kv head, blocks of HXQ_KV8_BLOCK = 64 tokens.
+ *   k        e4m3 [batch, n_kv_heads, n_blocks, 64, head_dim]   (OCP e4m3, no infinities)
+ *   v        e4m3 [batch, n_kv_heads, n_blocks, head_dim, 64]   (transposed in the block)
+ *   k_scale, v_scale  fp32 [batch, n_kv_heads, n_blocks]: value = e4m3 * scale
+ *   k_tail   [batch, n_kv_heads, 64, head_dim], v_tail [batch, n_kv_heads, head_dim, 64] in dtype
+ *            (HXQ_BF16 or HXQ_F16): the unfinished block, in 16 bits
+ *   blocks   int32 [batch, n_kv_heads, n_blocks]: place of the j-th block of a sequence and head
+ *            in its own n_blocks; NULL = j
+ * A sequence of `cached` tokens holds cached / 64 blocks in 8 bits and cached % 64 tokens in the
+ * tail.  A block is stored when its last token arrives: scale is the smallest power of two (2^-110
+ * at least) with max |x| <= 448 scale over the block's finite values, the stored value is x / scale
+ * rounded to nearest even; values that are not finite are stored as NaN.  Keys are rotated and both
+ * are rounded to dtype before, so that a cache holds the same bits however its tokens came: as one
+ * prompt, in pieces, or one by one.  A sequence with cached < 0 is skipped: nothing of it is read or
+ * written.  Tokens past n_blocks * 64 are not stored.
+ */
+#define HXQ_KV8_BLOCK 64
+typedef struct hxq_kv8 {
+    uint8_t *k;
+    uint8_t *v;
+    float *k_scale;
+    float *v_scale;
+    void *k_tail;
+    void *v_tail;
+    const int32_t *blocks;
+    int32_t dtype;
+    int32_t batch;
+    int32_t n_kv_heads;
+    int32_t head_dim;
+    int32_t n_blocks;
+} hxq_kv8;
+
+/*
+ * Rows of packed prompts into the cache.  Sequence s owns the rows cu_rows[s] .. cu_rows[s + 1]
+ * (device int32 [batch + 1]), which follow its cached[s] tokens; q and k are rotated to the
+ * positions pos[s], pos[s] + 1, ... (pos NULL = cached; rotate_half, inv_freq = theta^(-2i/D), the
+ * angle in 64 bits; theta 0 = no rotation).  dtype (q, k, v): any hxq_dtype.  q_out [rows, n_heads,
+ * D], k_out and v_out [rows, n_kv_heads, D] (contiguous, each optional): the rows in the cache's
+ * dtype, as the prompt's attention takes them.  cache->k NULL: no cache, the rows only (dtype,
+ * batch, n_kv_heads and head_dim are used).  `cached` is not advanced.
+ */
+int hxq_kv8_append(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
+                   int64_t k_row_stride, int64_t k_head_stride, const void *v,
+                   int64_t v_row_stride, int64_t v_head_stride, int32_t dtype,
+                   const int32_t *cu_rows, int64_t rows, int32_t n_heads, const int32_t *cached,
+                   const int32_t *pos, float theta, const hxq_kv8 *cache, void *q_out, void *k_out,
+                   void *v_out, hipStream_t stream);
+
+/*
+ * One token of each sequence: rotation (as hxq_kv8_append), its key and value into the cache, and
+ * its attention over the cached tokens and itself, out [batch, n_heads, D] (contiguous, any
+ * hxq_dtype).  Full blocks are read in 8 bits, the unfinished block and the token in 16 bits; the
+ * token that ends a block still sees it in 16 bits.  q keeps its fp32 bits after the rotation.
+ * weight_out (optional) fp32 [batch, n_kv_heads, n_blocks]: weight_in plus each block's share of
+ * the softmax, summed over the query heads of the kv head (entry j: the j-th block in order, the
+ * unfinished one included); weight_in NULL = zeros, weight_out may be weight_in.  A sequence with
+ * cached >= n_blocks * 64 has no room: its out is NaN, its cache and weights stay.  A block table
+ * entry outside [0, n_blocks) makes the sequence's out NaN.  workspace: device scratch of
+ * hxq_kv8_attn_decode_workspace_bytes(...) bytes, written and read within the call.
+ */
+int64_t hxq_kv8_attn_decode_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                                            int32_t head_dim, int32_t n_blocks, int32_t weights);
+int hxq_kv8_attn_decode(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
+                        int64_t k_row_stride, int64_t k_head_stride, const void *v,
+                        int64_t v_row_stride, int64_t v_head_stride, int32_t dtype,
+                        int32_t n_heads, const int32_t *cached, const int32_t *pos, float theta,
+                        float scale, const hxq_kv8 *cache, const float *weight_in,
+                        float *weight_out, void *out, int32_t out_dtype, void *workspace,
+                        int64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Eviction: of every sequence and kv head with more than `keep` full blocks (cached / 64), `keep`
+ * stay: the first `sink`, the last `recent`, and between them those of the greatest weight (ties to
+ * the lowest index; NaN counts as the greatest).  No cache data moves: blocks_out [batch,
+ * n_kv_heads, n_blocks] holds the blocks that stay in their order, then the others; weight_out the
+ * weights likewise, the unfinished block's behind those that stay, zero from there on; cached_out
+ * the new counts.  Outputs must not be the inputs.  blocks_in NULL = 0, 1, 2, ...
+ */
+int hxq_kv8_evict(const float *weight, const int32_t *blocks_in, const int32_t *cached,
+                  int32_t batch, int32_t n_kv_heads, int32_t n_blocks, int32_t keep, int32_t sink,
+                  int32_t recent, float *weight_out, int32_t *blocks_out, int32_t *cached_out,
+                  hipStream_t stream);
 
 /*
  * CDNAv3 encoder (k-means codebook, assignment, percentile sidecar), with the
