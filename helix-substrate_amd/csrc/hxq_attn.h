@@ -2,6 +2,8 @@
 // sequences, rotation.
 #pragma once
 
+#include <math.h>
+
 #include "hxq_common.h"
 
 namespace hxq {
@@ -55,10 +57,27 @@ __device__ __forceinline__ bool seq_tile(int n_seqs, int t, F count, int &seq, i
     return false;
 }
 
-// Turns per position of pair i of half pairs: theta^(-i / half) / 2 pi.  64 bits:
-// at position 10^5 an fp32 frequency is off by 10^5 2^-24 / 2 pi = 10^-3 turns.
-__device__ __forceinline__ double rope_turns(int i, int half, float theta) {
-    return exp2(-log2(static_cast<double>(theta)) * i / half) * 0.15915494309189533577;
+// Turns per position of pair i of D/2: theta^(-i / (D/2)) / 2 pi, in 64 bits (at position 10^5 an fp32
+// frequency is off by 10^5 2^-24 / 2 pi = 10^-3 turns).  p[k] = theta^(-2^k / (D/2)) comes from the
+// host: the power is six products, not a 64-bit exp and log in every launch.
+struct RopeTable {
+    double p[6];
+    bool on;
+};
+
+inline RopeTable rope_table(float theta, int head_dim) {
+    RopeTable t{};
+    t.on = theta > 0.f;
+    if (t.on)
+        for (int k = 0; k < 6; ++k) t.p[k] = pow(static_cast<double>(theta), -(1 << k) / (head_dim / 2.0));
+    return t;
+}
+
+__device__ __forceinline__ double rope_turns(const RopeTable &t, int i) {
+    double f = 0.15915494309189533577;
+#pragma unroll
+    for (int k = 0; k < 6; ++k) f *= i >> k & 1 ? t.p[k] : 1.0;
+    return f;
 }
 
 // cos and sin of pos * turns (in turns), reduced to half a turn in 64 bits.

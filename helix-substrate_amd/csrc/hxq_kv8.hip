@@ -41,6 +41,7 @@ template <bool BF16>
 __device__ __forceinline__ float up16(uint16_t v) { return BF16 ? bf16_to_f32(v) : f16_to_f32(v); }
 
 // maximum over the block; every thread gets it
+template <int THR>
 __device__ __forceinline__ float block_amax(float v, float *red) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, kWave));
@@ -49,20 +50,20 @@ __device__ __forceinline__ float block_amax(float v, float *red) {
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int i = 1; i < kThr / kWave; ++i) v = fmaxf(v, red[i]);
+    for (int i = 1; i < THR / kWave; ++i) v = fmaxf(v, red[i]);
     return v;
 }
 
 // One block's 64 * D values, in the order of the cache (rows of COLS values, PITCH apart in src), to
 // e4m3 and its scale.
-template <bool BF16, int D, int COLS, int PITCH>
+template <bool BF16, int D, int COLS, int PITCH, int THR>
 __device__ __forceinline__ void store_block(const uint16_t *src, uint8_t *dst, float *scale, float *red) {
-    constexpr int NC = kBlk * D / (16 * kThr);   // 16-value chunks a thread
+    constexpr int CH = kBlk * D / 16, NC = (CH + THR - 1) / THR;   // 16-value chunks, in all and a thread
     u32x4 x[NC][2];
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        const int c = threadIdx.x + i * kThr;
+        const int c = min(static_cast<int>(threadIdx.x) + i * THR, CH - 1);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             x[i][h] = *reinterpret_cast<const u32x4 *>(src + 16 * c / COLS * PITCH + 16 * c % COLS + 8 * h);
@@ -73,12 +74,13 @@ __device__ __forceinline__ void store_block(const uint16_t *src, uint8_t *dst, f
             }
         }
     }
-    top = block_amax(top, red);
+    top = block_amax<THR>(top, red);
     const int e = scale_exp(top);
     const float inv = pow2f(-e);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        const int c = threadIdx.x + i * kThr;
+        const int c = threadIdx.x + i * THR;
+        if (CH % THR && c >= CH) break;
         u32x4 w;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -121,7 +123,7 @@ __device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
 struct AppendArgs {
     HeadRows q, k, v;
     const int32_t *cu, *cached, *pos;
-    float theta;
+    RopeTable rope;
     int32_t rows, n_heads;
     hxq_kv8 c;
     void *q_out, *k_out, *v_out;
@@ -155,8 +157,8 @@ __global__ __launch_bounds__(kThr) void kv8_append_kernel(const AppendArgs a) {
     const int cached = a.cached[seq], held = cached % kBlk, full0 = cached / kBlk;
     const int total = held + n, last = (total - 1) / kBlk;
     const int pos0 = a.pos ? a.pos[seq] : cached;
-    const bool rope = a.theta > 0.f;
-    if (rope && threadIdx.x < HALF) turns[threadIdx.x] = rope_turns(threadIdx.x, HALF, a.theta);
+    const bool rope = a.rope.on;
+    if (rope && threadIdx.x < HALF) turns[threadIdx.x] = rope_turns(a.rope, threadIdx.x);
     __syncthreads();
     const int i0 = (threadIdx.x % TPR) * 8, r0 = threadIdx.x / TPR;
     const auto cos_sin = [&](int r, float (&c)[8], float (&s)[8]) {
@@ -258,8 +260,8 @@ __global__ __launch_bounds__(kThr) void kv8_append_kernel(const AppendArgs a) {
                 const int at = a.c.blocks ? a.c.blocks[bh * a.c.n_blocks + j] : j;
                 if (at >= 0 && at < a.c.n_blocks) {
                     const int64_t b = bh * a.c.n_blocks + at;
-                    store_block<BF16, D, D, D>(sk, a.c.k + b * kBlk * D, a.c.k_scale + b, red);
-                    store_block<BF16, D, kBlk, VP>(sv, a.c.v + b * kBlk * D, a.c.v_scale + b, red);
+                    store_block<BF16, D, D, D, kThr>(sk, a.c.k + b * kBlk * D, a.c.k_scale + b, red);
+                    store_block<BF16, D, kBlk, VP, kThr>(sv, a.c.v + b * kBlk * D, a.c.v_scale + b, red);
                 }
             } else {
                 // only the new tokens' slots: the others keep what they hold
@@ -283,21 +285,20 @@ __global__ __launch_bounds__(kThr) void kv8_append_kernel(const AppendArgs a) {
 struct DecodeArgs {
     HeadRows q, k, v;
     const int32_t *cached, *pos;
-    float theta, scale2;             // scale2 = scale * log2(e): the softmax is in powers of two
-    int32_t dtype, out_dtype, n_heads, splits;
+    RopeTable rope;
+    float scale2;                    // scale * log2(e): the softmax is in powers of two
+    int32_t out_dtype, n_heads, splits;
     hxq_kv8 c;
     const float *w_in;
     float *w_out;
     void *out;
-    float *part;                     // [batch * n_heads][splits][D + 2]: sums of p v, maximum, sum of p
-    float2 *share;                   // [batch * n_heads][n_blocks]: a block's sum of p and its maximum
+    float *part;                     // [batch * n_heads][splits][D]: sums of p v
+    float2 *ml;                      // [batch * n_heads][splits]: maximum of the scores, sum of p
+    float2 *share;                   // [batch * n_heads][n_blocks]: a block's sum of p and the maximum in it
 };
 
 constexpr int kHT = 8;               // query heads of a tile
-
-__device__ __forceinline__ float load_any(const void *p, int64_t i, int dt) {
-    return dt == HXQ_F32 ? load_act<HXQ_F32>(p, i) : dt == HXQ_BF16 ? load_act<HXQ_BF16>(p, i) : load_act<HXQ_F16>(p, i);
-}
+constexpr int kDThr = 512;           // 8 waves
 
 __device__ __forceinline__ void store_any(void *p, int64_t i, float v, int dt) {
     if (dt == HXQ_F32) store_act<HXQ_F32>(p, i, v);
@@ -306,9 +307,9 @@ __device__ __forceinline__ void store_any(void *p, int64_t i, float v, int dt) {
 }
 
 // A sequence's units: its full blocks and the unfinished one (with the new token), dealt to the
-// splits in runs of `per`.  At least 4 units a split, one for each wave.
+// splits in runs of `per`.  At least 8 units a split, one for each wave.
 __device__ __forceinline__ int units_per_split(int units, int splits) {
-    return max((units + splits - 1) / splits, kThr / kWave);
+    return max((units + splits - 1) / splits, kDThr / kWave);
 }
 
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -342,7 +343,7 @@ __device__ __forceinline__ float rows_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// One block: 4 waves over the units of a split of one (sequence, kv head, tile of 8 query heads).
+// One block: 8 waves over the units of a split of one (sequence, kv head, tile of 8 query heads).
 //
 // A wave takes a unit of 64 tokens by itself, in registers, with v_mfma_f32_16x16x32_bf16:
 //   S^T = K q^T: rows are tokens, columns are heads.  Row 4 k + r of tile j is given the token
@@ -354,10 +355,11 @@ __device__ __forceinline__ float rows_sum(float v) {
 // 16 columns hold 8 heads twice: q = hi + mid + lo in bf16 (24 bits; hi and mid in the two halves of
 // one operand, lo in a second), p = hi + lo (16 bits), their products added across the halves.  So q
 // keeps its fp32 bits and p 2^-17, at no cost where the cache's bytes bound the time.
-template <bool BF16, int D, bool W>
-__global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a) {
-    constexpr int HALF = D / 2, NC = D / 64, NT = D / 16, NW = kThr / kWave;
-    __shared__ __attribute__((aligned(16))) float sq[kHT][D];
+template <int DT, bool BF16, int D, bool W>
+__global__ __launch_bounds__(kDThr, 1) void kv8_decode_kernel(const DecodeArgs a) {
+    constexpr int HALF = D / 2, NC = D / 64, NT = D / 16, NW = kDThr / kWave;
+    constexpr int QP = D + 8, NP = ((kHT + 1) * HALF + kDThr - 1) / kDThr;   // pitch of q's rows; pairs a thread
+    __shared__ __attribute__((aligned(16))) uint16_t q_hm[2 * kHT][QP], q_lo[kHT][QP];   // hi | mid, lo
     __shared__ __attribute__((aligned(16))) uint16_t kn[D], vn[D];   // the new token
     __shared__ float cs[HALF], sn[HALF];
     __shared__ __attribute__((aligned(16))) float so[NW][kHT][D];
@@ -365,6 +367,17 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
     const int n_kv = a.c.n_kv_heads, group = a.n_heads / n_kv, htiles = (group + kHT - 1) / kHT;
     const int ht = blockIdx.y % htiles, kvh = blockIdx.y / htiles % n_kv, b = blockIdx.y / htiles / n_kv;
     const int h0 = kvh * group + ht * kHT, nh = min(kHT, group - ht * kHT);
+    // the new token's values are asked for first: they are needed first, and loads return in order
+    float x1[NP], x2[NP], xv = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int e = threadIdx.x + i * kDThr, h = min(e / HALF, kHT), hq = min(h, nh - 1);
+        const void *p = h == kHT ? a.k.p : a.q.p;
+        const int64_t at = (h == kHT ? b * a.k.row + kvh * a.k.head : b * a.q.row + (h0 + hq) * a.q.head) + e % HALF;
+        x1[i] = load_act<DT>(p, at);
+        x2[i] = load_act<DT>(p, at + HALF);
+    }
+    if (threadIdx.x < D) xv = load_act<DT>(a.v.p, b * a.v.row + kvh * a.v.head + threadIdx.x);
     const int cached = a.cached[b];
     if (cached < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -372,7 +385,7 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
     const int full = cached / kBlk, held = cached % kBlk, units = full + 1;
     if (full >= a.c.n_blocks) {      // no room
         if (blockIdx.x == 0)
-            for (int e = threadIdx.x; e < nh * D; e += kThr)
+            for (int e = threadIdx.x; e < nh * D; e += kDThr)
                 store_any(a.out, ((int64_t)b * a.n_heads + h0) * D + e, __uint_as_float(0x7fc00000u), a.out_dtype);
         return;
     }
@@ -381,33 +394,72 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
     const int64_t bh = (int64_t)b * n_kv + kvh;
     const int32_t *table = a.c.blocks ? a.c.blocks + bh * a.c.n_blocks : nullptr;
 
-    // the new token: rotation, in fp32
-    const bool rope = a.theta > 0.f;
-    if (rope && threadIdx.x < HALF)
-        rope_cs(a.pos ? a.pos[b] : cached, rope_turns(threadIdx.x, HALF, a.theta), cs[threadIdx.x], sn[threadIdx.x]);
-    __syncthreads();
-    for (int e = threadIdx.x; e < (kHT + 1) * HALF; e += kThr) {
-        const int h = e / HALF, i = e % HALF;
-        float y1 = 0.f, y2 = 0.f;
-        if (h < nh || h == kHT) {
-            const void *p = h == kHT ? a.k.p : a.q.p;
-            const int64_t at = (h == kHT ? b * a.k.row + kvh * a.k.head : b * a.q.row + (h0 + h) * a.q.head) + i;
-            const float x1 = load_any(p, at, a.dtype), x2 = load_any(p, at + HALF, a.dtype);
-            y1 = rope ? x1 * cs[i] - x2 * sn[i] : x1;
-            y2 = rope ? x2 * cs[i] + x1 * sn[i] : x2;
-        }
-        if (h < kHT) {
-            sq[h][i] = y1;
-            sq[h][i + HALF] = y2;
-        } else {
-            const uint32_t w = pack16<BF16>(y1, y2);
-            kn[i] = static_cast<uint16_t>(w);
-            kn[i + HALF] = static_cast<uint16_t>(w >> 16);
-        }
+    // A unit's bytes: K of step (j, c) and V of 16 dimensions, 16 bytes a lane.  They are asked for
+    // one unit ahead, K when the scores no longer need its registers, V after the second product.
+    const int uf = min(u1, full);
+    u32x4 kr[4][NC], vr[NT];
+    float ks = 1.f, vs = 1.f, bad = 0.f;
+    int64_t blk = 0;
+    const auto find = [&](int u) {
+        int at = table ? table[u] : u;
+        bad = at < 0 || at >= a.c.n_blocks ? __uint_as_float(0x7fc00000u) : 0.f;
+        blk = bh * a.c.n_blocks + min(max(at, 0), a.c.n_blocks - 1);
+    };
+    const auto load_k = [&] {
+        const u32x4 *kp = reinterpret_cast<const u32x4 *>(a.c.k + blk * kBlk * D);
+        ks = a.c.k_scale[blk];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) kr[j][c] = kp[((lh >> 2) * 16 + 4 * j + (lh & 3)) * (D / 16) + 4 * c + kq];
+    };
+    const auto load_v = [&] {
+        const u32x4 *vp = reinterpret_cast<const u32x4 *>(a.c.v + blk * kBlk * D);
+        vs = a.c.v_scale[blk];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) vr[i] = vp[(16 * i + lh) * 4 + kq];
+    };
+    if (u0 + wave < uf) {
+        find(u0 + wave);
+        load_k();
+        load_v();
     }
-    for (int e = threadIdx.x; e < D; e += kThr)
-        vn[e] = static_cast<uint16_t>(pack16<BF16>(load_any(a.v.p, b * a.v.row + kvh * a.v.head + e, a.dtype), 0.f));
-    __syncthreads();
+
+    // the new token: rotation in fp32, q in three bf16 (24 bits)
+    const bool rope = a.rope.on;
+    if (rope && threadIdx.x < HALF)
+        rope_cs(a.pos ? a.pos[b] : cached, rope_turns(a.rope, threadIdx.x), cs[threadIdx.x], sn[threadIdx.x]);
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int e = threadIdx.x + i * kDThr, h = e / HALF, d = e % HALF;
+        if (h > kHT) break;
+        float y1 = x1[i], y2 = x2[i];
+        if (rope) {
+            y1 = x1[i] * cs[d] - x2[i] * sn[d];
+            y2 = x2[i] * cs[d] + x1[i] * sn[d];
+        }
+        if (h == kHT) {
+            const uint32_t w = pack16<BF16>(y1, y2);
+            kn[d] = static_cast<uint16_t>(w);
+            kn[d + HALF] = static_cast<uint16_t>(w >> 16);
+            continue;
+        }
+        if (h >= nh) y1 = y2 = 0.f;
+        const uint32_t hi = pack16<true>(y1, y2);
+        y1 -= __uint_as_float(hi << 16);
+        y2 -= __uint_as_float(hi & 0xffff0000u);
+        const uint32_t mid = pack16<true>(y1, y2);
+        const uint32_t lo = pack16<true>(y1 - __uint_as_float(mid << 16), y2 - __uint_as_float(mid & 0xffff0000u));
+        q_hm[h][d] = static_cast<uint16_t>(hi);
+        q_hm[h][d + HALF] = static_cast<uint16_t>(hi >> 16);
+        q_hm[h + kHT][d] = static_cast<uint16_t>(mid);
+        q_hm[h + kHT][d + HALF] = static_cast<uint16_t>(mid >> 16);
+        q_lo[h][d] = static_cast<uint16_t>(lo);
+        q_lo[h][d + HALF] = static_cast<uint16_t>(lo >> 16);
+    }
+    if (threadIdx.x < D) vn[threadIdx.x] = static_cast<uint16_t>(pack16<BF16>(xv, 0.f));
+    lds_barrier();
 
     // q as B operands: d = 64 c + 16 kq + 8 e + 0..7 of step (c, e), as the 16-byte loads of K give it
     u32x4 q1[NC][2], q2[NC][2];
@@ -415,20 +467,10 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
     for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float *p = &sq[lh & 7][64 * c + 16 * kq + 8 * e];
-            float hi[8], mid[8], lo[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                hi[j] = p[j];
-                mid[j] = hi[j] - bf16_to_f32(f32_to_bf16(hi[j]));
-                lo[j] = mid[j] - bf16_to_f32(f32_to_bf16(mid[j]));
-                if (lh >= 8) {
-                    hi[j] = mid[j];
-                    lo[j] = 0.f;
-                }
-            }
-            q1[c][e] = pack8<true>(hi);
-            q2[c][e] = pack8<true>(lo);
+            const int d = 64 * c + 16 * kq + 8 * e;
+            q1[c][e] = *reinterpret_cast<const u32x4 *>(&q_hm[lh][d]);
+            q2[c][e] = *reinterpret_cast<const u32x4 *>(&q_lo[lh & 7][d]);
+            if (lh >= kHT) q2[c][e] = u32x4{0u, 0u, 0u, 0u};
         }
 
     f32x4 o[NT];
@@ -481,22 +523,9 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
         }
     };
 
-    const int uf = min(u1, full);
     for (int u = u0 + wave; u < uf; u += NW) {
-        int at = table ? table[u] : u;
-        const float bad = at < 0 || at >= a.c.n_blocks ? __uint_as_float(0x7fc00000u) : 0.f;
-        at = min(max(at, 0), a.c.n_blocks - 1);
-        const int64_t blk = bh * a.c.n_blocks + at;
-        const u32x4 *kp = reinterpret_cast<const u32x4 *>(a.c.k + blk * kBlk * D);
-        const u32x4 *vp = reinterpret_cast<const u32x4 *>(a.c.v + blk * kBlk * D);
-        const float ks = a.c.k_scale[blk], vs = a.c.v_scale[blk];
-        u32x4 kr[4][NC], vr[NT];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) kr[j][c] = kp[((lh >> 2) * 16 + 4 * j + (lh & 3)) * (D / 16) + 4 * c + kq];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) vr[i] = vp[(16 * i + lh) * 4 + kq];
+        const bool more = u + NW < uf;
+        const float bad_now = bad;
         f32x4 s[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -510,12 +539,17 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
                     s[j] = mfma16(k8, q2[c][e], s[j]);
                 }
         }
+        if (more) {
+            find(u + NW);
+            load_k();
+        }
         u32x4 p[2];
-        soften(s, u, bad, kBlk, p);
+        soften(s, u, bad_now, kBlk, p);
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) o[i] = mfma16(e4m3_bf16(vr[i][2 * e], vr[i][2 * e + 1], vs), p[e], o[i]);
+        if (more) load_v();
     }
 
     // the unfinished block in 16 bits, its last token from shared memory; fp16 as the sum of two bf16
@@ -531,20 +565,30 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
         }
     };
     if (tail && wave == (full - u0) % NW) {
+        // every slot is asked for at once; what is behind the last token is dropped afterwards
+        u32x4 kt[4][NC][2], vt[NT][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    kt[j][c][e] = *reinterpret_cast<const u32x4 *>(k_tail + ((lh >> 2) * 16 + 4 * j + (lh & 3)) * D + 64 * c + 16 * kq + 8 * e);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) vt[i][e] = *reinterpret_cast<const u32x4 *>(v_tail + (16 * i + lh) * kBlk + 16 * kq + 8 * e);
         f32x4 s[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             s[j] = f32x4{0.f, 0.f, 0.f, 0.f};
             const int t = (lh >> 2) * 16 + 4 * j + (lh & 3);
-            const uint16_t *row = k_tail + t * D;
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int d = 64 * c + 16 * kq + 8 * e;
-                    u32x4 w = u32x4{0u, 0u, 0u, 0u};
-                    if (t < held) w = *reinterpret_cast<const u32x4 *>(row + d);
-                    else if (t == held) w = *reinterpret_cast<const u32x4 *>(kn + d);
+                    u32x4 w = kt[j][c][e];
+                    if (t == held) w = *reinterpret_cast<const u32x4 *>(kn + 64 * c + 16 * kq + 8 * e);
                     if constexpr (BF16) {
                         s[j] = mfma16(w, q1[c][e], s[j]);
                         s[j] = mfma16(w, q2[c][e], s[j]);
@@ -564,13 +608,13 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int d = 16 * i + lh, t0 = 16 * kq + 8 * e;
-                u32x4 w = u32x4{0u, 0u, 0u, 0u};
-                if (t0 < held) w = *reinterpret_cast<const u32x4 *>(v_tail + d * kBlk + t0);
+                const uint32_t nv = vn[d];
+                u32x4 w = vt[i][e];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int t = t0 + 2 * j;
-                    const uint32_t x = t < held ? w[j] & 0xffffu : t == held ? vn[d] : 0u;
-                    const uint32_t y = t + 1 < held ? w[j] >> 16 : t + 1 == held ? vn[d] : 0u;
+                    const uint32_t x = t < held ? w[j] & 0xffffu : t == held ? nv : 0u;
+                    const uint32_t y = t + 1 < held ? w[j] >> 16 : t + 1 == held ? nv : 0u;
                     w[j] = x | y << 16;
                 }
                 if constexpr (BF16) {
@@ -584,7 +628,7 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
             }
     }
 
-    // the four waves' results
+    // the waves' results
     l = rows_sum(l);
     if (kq == 0 && lh < kHT) {
         sm[wave][lh] = m;
@@ -599,7 +643,7 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
     }
     __syncthreads();
     const bool alone = per >= units;
-    for (int e = threadIdx.x; e < nh * D; e += kThr) {
+    for (int e = threadIdx.x; e < nh * D; e += kDThr) {
         const int h = e / D, d = e % D;
         float mm = sm[0][h];
 #pragma unroll
@@ -613,19 +657,13 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
         }
         const int64_t row = (int64_t)b * a.n_heads + h0 + h;
         if (alone) store_any(a.out, row * D + d, x / ll, a.out_dtype);
-        if (!alone || W) {
-            float *pt = a.part + (row * a.splits + blockIdx.x) * (D + 2);
-            pt[d] = x;
-            if (d == 0) {
-                pt[D] = mm;
-                pt[D + 1] = ll;
-            }
-        }
+        else a.part[(row * a.splits + blockIdx.x) * D + d] = x;
+        if ((!alone || W) && d == 0) a.ml[row * a.splits + blockIdx.x] = float2{mm, ll};
     }
 
     // the token into the cache (no other block of the launch reads its place)
     if (!tail || ht != 0) return;
-    for (int e = threadIdx.x; e < D; e += kThr) {
+    for (int e = threadIdx.x; e < D; e += kDThr) {
         k_tail[held * D + e] = kn[e];
         v_tail[e * kBlk + held] = vn[e];
     }
@@ -633,74 +671,86 @@ __global__ __launch_bounds__(kThr, 2) void kv8_decode_kernel(const DecodeArgs a)
     const int at = table ? table[full] : full;
     if (at < 0 || at >= a.c.n_blocks) return;
     __syncthreads();
-    const int64_t blk = bh * a.c.n_blocks + at;
-    store_block<BF16, D, D, D>(k_tail, a.c.k + blk * kBlk * D, a.c.k_scale + blk, red);
-    store_block<BF16, D, kBlk, kBlk>(v_tail, a.c.v + blk * kBlk * D, a.c.v_scale + blk, red);
+    blk = bh * a.c.n_blocks + at;
+    store_block<BF16, D, D, D, kDThr>(k_tail, a.c.k + blk * kBlk * D, a.c.k_scale + blk, red);
+    store_block<BF16, D, kBlk, kBlk, kDThr>(v_tail, a.c.v + blk * kBlk * D, a.c.v_scale + blk, red);
 }
 
-constexpr int kJoin = 1024;
-
-// The splits' results of one query head (grid.x = batch * n_heads), joined.
-template <int D>
-__global__ __launch_bounds__(kJoin) void kv8_join_kernel(const DecodeArgs a) {
-    constexpr int NG = kJoin / D;
-    __shared__ float sx[NG][D], sl[NG];
-    const int64_t row = blockIdx.x;
-    const int cached = a.cached[row / a.n_heads];
-    if (cached < 0 || cached / kBlk >= a.c.n_blocks) return;
-    const int units = cached / kBlk + 1, per = units_per_split(units, a.splits);
-    const int n = (units + per - 1) / per;
-    if (n == 1) return;    // written already
-    const float *pt = a.part + row * a.splits * (D + 2);
-    float mm = -INFINITY;
-    for (int i = 0; i < n; ++i) mm = fmaxf(mm, pt[(int64_t)i * (D + 2) + D]);
-    const int d = threadIdx.x % D, g = threadIdx.x / D;
-    float x = 0.f, ll = 0.f;
-    for (int i = g; i < n; i += NG) {
-        const float *p = pt + (int64_t)i * (D + 2);
-        const float f = __builtin_amdgcn_exp2f(p[D] - mm);
-        x = fmaf(f, p[d], x);
-        ll = fmaf(f, p[D + 1], ll);
-    }
-    sx[g][d] = x;
-    if (d == 0) sl[g] = ll;
-    __syncthreads();
-    if (g) return;
+// The maximum and the sum over all splits of one query head's scores, by a wave.
+__device__ __forceinline__ float2 join_ml(const float2 *ml, int n) {
+    const int lane = threadIdx.x & 63;
+    float mm = -INFINITY, ll = 0.f;
+    for (int i = lane; i < n; i += kWave) mm = fmaxf(mm, ml[i].x);
 #pragma unroll
-    for (int i = 1; i < NG; ++i) {
-        x += sx[i][d];
-        ll += sl[i];
-    }
-    store_any(a.out, row * D + d, x / ll, a.out_dtype);
+    for (int s = 32; s >= 1; s >>= 1) mm = fmaxf(mm, __shfl_xor(mm, s, kWave));
+    for (int i = lane; i < n; i += kWave) ll = fmaf(__builtin_amdgcn_exp2f(ml[i].x - mm), ml[i].y, ll);
+    return float2{mm, wave_sum(ll)};
 }
 
-// weight_out = weight_in + every block's share, one (sequence, kv head) per blockIdx.y, kThr blocks
-// of the cache per blockIdx.x.
+// What is left when the splits are done.  Blocks below batch * n_heads: one query head's splits
+// joined.  The others: weight_out = weight_in + every cache block's share of the softmax, kThr cache
+// blocks of one (sequence, kv head) each.
 template <int D>
-__global__ __launch_bounds__(kThr) void kv8_share_kernel(const DecodeArgs a) {
-    __shared__ float red[kThr / kWave];
-    const int n_kv = a.c.n_kv_heads, group = a.n_heads / n_kv;
-    const int64_t bh = blockIdx.y;
+__global__ __launch_bounds__(kThr) void kv8_join_kernel(const DecodeArgs a) {
+    constexpr int Q = D / 4, NG = kThr / Q, NW = kThr / kWave;
+    __shared__ __attribute__((aligned(16))) float sx[NG][D];
+    __shared__ float2 tot[64];
+    const int n_kv = a.c.n_kv_heads, group = a.n_heads / n_kv, n_rows = a.c.batch * a.n_heads;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const auto splits_of = [&](int units) {
+        const int per = units_per_split(units, a.splits);
+        return (units + per - 1) / per;
+    };
+    if (static_cast<int>(blockIdx.x) < n_rows) {
+        const int64_t row = blockIdx.x;
+        const int cached = a.cached[row / a.n_heads];
+        if (cached < 0 || cached / kBlk >= a.c.n_blocks) return;
+        const int n = splits_of(cached / kBlk + 1);
+        if (n == 1) return;    // written already
+        const float2 *ml = a.ml + row * a.splits;
+        const float2 t = join_ml(ml, n);
+        const float *pt = a.part + row * a.splits * D;
+        const int d = threadIdx.x % Q * 4, g = threadIdx.x / Q;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int i = g; i < n; i += NG) {
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - t.x);
+            const f32x4 p = *reinterpret_cast<const f32x4 *>(pt + (int64_t)i * D + d);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = fmaf(f, p[r], x[r]);
+        }
+        *reinterpret_cast<f32x4 *>(&sx[g][d]) = x;
+        __syncthreads();
+        if (threadIdx.x >= D) return;
+        float y = 0.f;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) y += sx[i][threadIdx.x];
+        store_any(a.out, row * D + threadIdx.x, y / t.y, a.out_dtype);
+        return;
+    }
+    const int chunks = (a.c.n_blocks + kThr - 1) / kThr, id = blockIdx.x - n_rows;
+    const int64_t bh = id / chunks;
     const int b = static_cast<int>(bh / n_kv), kvh = static_cast<int>(bh % n_kv);
     const int cached = a.cached[b];
     if (cached < 0) return;
     const int units = cached / kBlk < a.c.n_blocks ? cached / kBlk + 1 : 0;   // no room: the weights stay
-    const int per = units_per_split(units, a.splits), n = (units + per - 1) / per;
-    const int j = blockIdx.x * kThr + threadIdx.x;
+    const int n = splits_of(units), j = id % chunks * kThr + threadIdx.x;
+    const int64_t row0 = (int64_t)b * a.n_heads + kvh * group;
     float w = 0.f;
-    for (int g = 0; g < (units ? group : 0); ++g) {
-        const int64_t row = (int64_t)b * a.n_heads + kvh * group + g;
-        const float *pt = a.part + row * a.splits * (D + 2);
-        float mm = -INFINITY;
-        for (int i = threadIdx.x; i < n; i += kThr) mm = fmaxf(mm, pt[(int64_t)i * (D + 2) + D]);
-        mm = block_amax(mm, red);
-        float ll = 0.f;
-        for (int i = 0; i < n; ++i)
-            ll = fmaf(__builtin_amdgcn_exp2f(pt[(int64_t)i * (D + 2) + D] - mm), pt[(int64_t)i * (D + 2) + D + 1], ll);
-        if (j < units) {
-            const float2 s = a.share[row * a.c.n_blocks + j];
-            w += s.x * __builtin_amdgcn_exp2f(s.y - mm) / ll;
+    for (int g0 = 0; g0 < (units ? group : 0); g0 += 64) {
+        const int ng = min(group - g0, 64);
+        __syncthreads();
+        for (int g = wave; g < ng; g += NW) {
+            const float2 t = join_ml(a.ml + (row0 + g0 + g) * a.splits, n);
+            if (lane == 0) tot[g] = float2{t.x, 1.f / t.y};
         }
+        __syncthreads();
+        if (j < units)
+#pragma unroll 8
+            for (int g = 0; g < ng; ++g) {
+                const float2 s = a.share[(row0 + g0 + g) * a.c.n_blocks + j];
+                w = fmaf(s.x * __builtin_amdgcn_exp2f(s.y - tot[g].x), tot[g].y, w);
+            }
     }
     if (j < a.c.n_blocks) a.w_out[bh * a.c.n_blocks + j] = (a.w_in ? a.w_in[bh * a.c.n_blocks + j] : 0.f) + w;
 }
@@ -822,20 +872,47 @@ bool kv8_ok(const hxq_kv8 *c, bool need) {
            c->n_blocks <= (1 << 24);
 }
 
-// Splits of one sequence's cache: about two blocks of 4 waves for each compute unit over the whole
-// launch, and no more than leave each wave a unit.
+// go(row dtype, cache in bf16, head_dim) as constants
+template <typename F>
+void kv8_dispatch(int32_t dtype, const hxq_kv8 &c, F go) {
+    const auto by_d = [&](auto dt, auto bf) {
+        if (c.head_dim == 128) go(dt, bf, std::integral_constant<int, 128>{});
+        else go(dt, bf, std::integral_constant<int, 64>{});
+    };
+    const auto by_c = [&](auto dt) {
+        if (c.dtype == HXQ_BF16) by_d(dt, std::true_type{});
+        else by_d(dt, std::false_type{});
+    };
+    if (dtype == HXQ_F32) by_c(std::integral_constant<int, HXQ_F32>{});
+    else if (dtype == HXQ_BF16) by_c(std::integral_constant<int, HXQ_BF16>{});
+    else by_c(std::integral_constant<int, HXQ_F16>{});
+}
+
+// Splits of one sequence's cache: enough for 4 blocks a compute unit (sequences of different lengths
+// even out), down to 16 units each, two for a wave; where that leaves compute units idle, down to 8.
 int kv8_splits(int64_t tiles, int32_t n_blocks) {
-    const int64_t want = (2 * device_cu_count() + tiles - 1) / tiles;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, (n_blocks + 3) / 4)));
+    const int64_t cus = device_cu_count();
+    const int64_t even = std::min<int64_t>((4 * cus + tiles - 1) / tiles, (n_blocks + 15) / 16);
+    const int64_t idle = std::min<int64_t>((cus + tiles - 1) / tiles, (n_blocks + 7) / 8);
+    return static_cast<int>(std::max<int64_t>(1, std::max(even, idle)));
 }
 
 int64_t kv8_tiles(int32_t batch, int32_t n_heads, int32_t n_kv) {
     return (int64_t)batch * n_kv * ((n_heads / n_kv + kHT - 1) / kHT);
 }
 
-int64_t kv8_part_bytes(int32_t batch, int32_t n_heads, int splits, int32_t D, bool weights) {
-    if (splits == 1 && !weights) return 0;
-    return ((int64_t)batch * n_heads * splits * (D + 2) * 4 + 15) / 16 * 16;
+// Workspace: part, then ml, then share.
+struct Kv8Ws {
+    int64_t ml, share, bytes;
+};
+
+Kv8Ws kv8_ws(int32_t batch, int32_t n_heads, int splits, int32_t D, int32_t n_blocks, bool weights) {
+    const int64_t rows = (int64_t)batch * n_heads;
+    Kv8Ws w;
+    w.ml = splits > 1 ? rows * splits * D * 4 : 0;
+    w.share = w.ml + (splits > 1 || weights ? (rows * splits * 8 + 15) / 16 * 16 : 0);
+    w.bytes = w.share + (weights ? rows * n_blocks * 8 : 0);
+    return w;
 }
 
 }  // namespace
@@ -858,26 +935,15 @@ extern "C" int hxq_kv8_append(const void *q, int64_t q_row_stride, int64_t q_hea
     for (const void *p : {q_out, k_out, v_out})
         HXQ_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "outputs must be 16-byte aligned");
     if (rows == 0) return HXQ_OK;
-    const AppendArgs a{qr, kr, vr, cu_rows, cached, pos, theta, static_cast<int32_t>(rows), n_heads, *cache, q_out, k_out, v_out};
+    const AppendArgs a{qr, kr, vr, cu_rows, cached, pos, rope_table(theta, cache->head_dim), static_cast<int32_t>(rows), n_heads, *cache, q_out, k_out, v_out};
     const int64_t tiles = rows / kBlk + 2 * (int64_t)cache->batch;
     const int64_t heads = cache->n_kv_heads + (q_out ? (n_heads + kQHeads - 1) / kQHeads : 0);
     HXQ_REQUIRE(tiles < (int64_t{1} << 31) && heads <= 65535, "too many rows or heads");
     const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(heads));
-    const auto go = [&](auto dt, auto bf, auto d) {
+    kv8_dispatch(dtype, *cache, [&](auto dt, auto bf, auto d) {
         hipLaunchKernelGGL((kv8_append_kernel<decltype(dt)::value, decltype(bf)::value, decltype(d)::value>), grid,
                            dim3(kThr), 0, stream, a);
-    };
-    const auto by_d = [&](auto dt, auto bf) {
-        if (cache->head_dim == 128) go(dt, bf, std::integral_constant<int, 128>{});
-        else go(dt, bf, std::integral_constant<int, 64>{});
-    };
-    const auto by_c = [&](auto dt) {
-        if (cache->dtype == HXQ_BF16) by_d(dt, std::true_type{});
-        else by_d(dt, std::false_type{});
-    };
-    if (dtype == HXQ_F32) by_c(std::integral_constant<int, HXQ_F32>{});
-    else if (dtype == HXQ_BF16) by_c(std::integral_constant<int, HXQ_BF16>{});
-    else by_c(std::integral_constant<int, HXQ_F16>{});
+    });
     HXQ_LAUNCH_CHECK();
     return HXQ_OK;
 }
@@ -886,8 +952,7 @@ extern "C" int64_t hxq_kv8_attn_decode_workspace_bytes(int32_t batch, int32_t n_
                                                        int32_t head_dim, int32_t n_blocks, int32_t weights) {
     if (batch <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_blocks <= 0) return -1;
     const int s = kv8_splits(kv8_tiles(batch, n_heads, n_kv_heads), n_blocks);
-    return kv8_part_bytes(batch, n_heads, s, head_dim, weights != 0) +
-           (weights ? (int64_t)batch * n_heads * n_blocks * 8 : 0);
+    return kv8_ws(batch, n_heads, s, head_dim, n_blocks, weights != 0).bytes;
 }
 
 extern "C" int hxq_kv8_attn_decode(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
@@ -906,33 +971,28 @@ extern "C" int hxq_kv8_attn_decode(const void *q, int64_t q_row_stride, int64_t 
     const int64_t tiles = kv8_tiles(cache->batch, n_heads, cache->n_kv_heads);
     HXQ_REQUIRE(tiles <= 65535 && (int64_t)cache->batch * n_heads < (int64_t{1} << 31), "batch * heads too large");
     const int splits = kv8_splits(tiles, cache->n_blocks);
-    const int64_t part = kv8_part_bytes(cache->batch, n_heads, splits, cache->head_dim, weight_out != nullptr);
-    const int64_t need = hxq_kv8_attn_decode_workspace_bytes(cache->batch, n_heads, cache->n_kv_heads, cache->head_dim,
-                                                             cache->n_blocks, weight_out != nullptr);
-    HXQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+    const Kv8Ws w = kv8_ws(cache->batch, n_heads, splits, cache->head_dim, cache->n_blocks, weight_out != nullptr);
+    HXQ_REQUIRE(w.bytes == 0 || (workspace && workspace_bytes >= w.bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "workspace too small or not 16-byte aligned");
+    char *ws = static_cast<char *>(workspace);
     const DecodeArgs a{{q, q_row_stride, q_head_stride}, {k, k_row_stride, k_head_stride}, {v, v_row_stride, v_head_stride},
-                       cached, pos, theta, scale * 1.44269504088896340736f, dtype, out_dtype, n_heads, splits, *cache,
-                       weight_in, weight_out, out, static_cast<float *>(workspace),
-                       reinterpret_cast<float2 *>(static_cast<char *>(workspace) + part)};
+                       cached, pos, rope_table(theta, cache->head_dim), scale * 1.44269504088896340736f, out_dtype, n_heads, splits, *cache,
+                       weight_in, weight_out, out, reinterpret_cast<float *>(ws),
+                       reinterpret_cast<float2 *>(ws + w.ml), reinterpret_cast<float2 *>(ws + w.share)};
+    // what the second launch has to do: rows to join, chunks of weights
+    const int64_t rows = (int64_t)cache->batch * n_heads;
+    const int64_t chunks = weight_out ? (int64_t)cache->batch * cache->n_kv_heads * ((cache->n_blocks + kThr - 1) / kThr) : 0;
+    HXQ_REQUIRE(rows + chunks < (int64_t{1} << 31), "batch * heads or blocks too large");
+    const dim3 join(static_cast<uint32_t>(rows + chunks));
     const dim3 grid(splits, static_cast<uint32_t>(tiles));
-    const auto go = [&](auto bf, auto dd) {
+    const auto go = [&](auto dt, auto bf, auto dd) {
+        constexpr int T = decltype(dt)::value, D = decltype(dd)::value;
         constexpr bool B = decltype(bf)::value;
-        constexpr int D = decltype(dd)::value;
-        if (weight_out) hipLaunchKernelGGL((kv8_decode_kernel<B, D, true>), grid, dim3(kThr), 0, stream, a);
-        else hipLaunchKernelGGL((kv8_decode_kernel<B, D, false>), grid, dim3(kThr), 0, stream, a);
-        if (splits > 1)
-            hipLaunchKernelGGL((kv8_join_kernel<D>), dim3(cache->batch * n_heads), dim3(kJoin), 0, stream, a);
-        if (weight_out)
-            hipLaunchKernelGGL((kv8_share_kernel<D>), dim3((cache->n_blocks + kThr - 1) / kThr, cache->batch * cache->n_kv_heads),
-                               dim3(kThr), 0, stream, a);
+        if (weight_out) hipLaunchKernelGGL((kv8_decode_kernel<T, B, D, true>), grid, dim3(kDThr), 0, stream, a);
+        else hipLaunchKernelGGL((kv8_decode_kernel<T, B, D, false>), grid, dim3(kDThr), 0, stream, a);
+        if (splits > 1 || weight_out) hipLaunchKernelGGL((kv8_join_kernel<D>), join, dim3(kThr), 0, stream, a);
     };
-    const auto by_d = [&](auto bf) {
-        if (cache->head_dim == 128) go(bf, std::integral_constant<int, 128>{});
-        else go(bf, std::integral_constant<int, 64>{});
-    };
-    if (cache->dtype == HXQ_BF16) by_d(std::true_type{});
-    else by_d(std::false_type{});
+    kv8_dispatch(dtype, *cache, go);
     HXQ_LAUNCH_CHECK();
     return HXQ_OK;
 }

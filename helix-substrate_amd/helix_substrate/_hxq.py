@@ -812,64 +812,72 @@ def attn_rope_decode(qkv, pos, n_heads, n_kv, head_dim, theta, k_cache, v_cache,
 KV8_BLOCK = 64
 
 
-def _need_heads_of(**named):
-    """q, k, v, out: [rows, heads, head_dim] views on one device, head_dim contiguous (any row and
-    head stride that the library takes); returns the device."""
-    dev = index = None
-    for name, t in named.items():
-        if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+# The wrappers below are called once a layer and token: one condition over everything that has to
+# hold, and the reason looked for only where it does not.
+def _why(device, rows=(), plain=()):
+    """Raise for the tensor that does not fit: device tensors on one device, row views [rows, heads,
+    head_dim] with head_dim contiguous, the others contiguous."""
+    for name, t in rows:
+        if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
             raise ValueError(f"{name} must be [rows, heads, head_dim] with head_dim contiguous")
-        i = t.get_device()
-        if i < 0 or not t.is_cuda:
+    for name, t in (*rows, *plain):
+        if t is not None and t.get_device() < 0:
             raise RuntimeError("HXQ kernels take device tensors only")
-        if dev is None:
-            dev, index = t.device, i
-        elif i != index:
-            raise RuntimeError(f"tensors on different devices: {dev} vs {t.device}")
-    return dev
+        if t is not None and t.get_device() != device:
+            raise RuntimeError(f"{name} is on {t.device}, not on cuda:{device}")
+    for name, t in plain:
+        if t is not None and not t.is_contiguous():
+            raise RuntimeError(f"{name} must be contiguous")
 
 
-def _view(t):
-    """Pointer, row stride and head stride; strides that no element needs count as 0."""
-    r, h, _ = t.shape
-    return t.data_ptr(), t.stride(0) if r > 1 else 0, t.stride(1) if h > 1 else 0
+def _flat(t, device):
+    return t is None or (t.get_device() == device and t.is_contiguous())
 
 
-def _on(t):
-    """The current device for the call when it is not the tensor's (the library asks it for its
-    compute units)."""
-    return torch.cuda.device(t.device) if torch.cuda.current_device() != t.get_device() else None
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _kv8_call(t, name, *args):
-    fn, dev = getattr(lib(), name), _on(t)
-    if dev is None:
-        _check(name, fn(*args))
+def _call_on(device, name, *args):
+    """Call with `device` current: the library counts its compute units."""
+    fn = getattr(_lib or lib(), name)
+    if _get_device() == device:
+        rc = fn(*args)
     else:
-        with dev:
-            _check(name, fn(*args))
+        with torch.cuda.device(device):
+            rc = fn(*args)
+    if rc:
+        _check(name, rc)
 
 
 def attn_prompt(q, k, v, cu_q, cu_k, scale, causal, out):
     """Attention of packed prompts (hxq_attn_prompt): q [rows, heads, D], k and v [rows, kv heads,
     D], bf16 or fp16, cu_* int32 [n_seqs + 1]; out as q."""
-    dev = _need_heads_of(q=q, k=k, v=v, out=out)
-    if not q.dtype == k.dtype == v.dtype == out.dtype:
-        raise RuntimeError(f"q, k, v and out must have one dtype (got {q.dtype}, {k.dtype}, "
-                           f"{v.dtype}, {out.dtype})")
-    if k.shape != v.shape or k.shape[2] != q.shape[2] or out.shape != q.shape:
+    dev, qs, ks, dt = q.get_device(), q.shape, k.shape, q.dtype
+    qt, kt, vt, ot = q.stride(), k.stride(), v.stride(), out.stride()
+    if not (len(qs) == len(ks) == 3 and qt[2] == kt[-1] == vt[-1] == ot[-1] == 1 and dev >= 0
+            and k.get_device() == v.get_device() == out.get_device() == dev
+            and _flat(cu_q, dev) and _flat(cu_k, dev)):
+        _why(dev, (("q", q), ("k", k), ("v", v), ("out", out)), (("cu_q", cu_q), ("cu_k", cu_k)))
+    if not dt == k.dtype == v.dtype == out.dtype:
+        raise RuntimeError(f"q, k, v and out must have one dtype (got {dt}, {k.dtype}, {v.dtype}, "
+                           f"{out.dtype})")
+    if ks != v.shape or ks[2] != qs[2] or out.shape != qs:
         raise ValueError("shapes must be q, out [rows, heads, D], k, v [rows, kv heads, D]")
     _need_i32(cu_q=cu_q, cu_k=cu_k)
-    if _need_device(cu_q, cu_k) != dev:
-        raise RuntimeError("tensors on different devices")
     if cu_q.dim() != 1 or cu_q.numel() < 1 or (cu_k is not None and cu_k.shape != cu_q.shape):
         raise ValueError("cu_q and cu_k must be [n_seqs + 1]")
-    if cu_k is None and k.shape[0] != q.shape[0]:
+    if cu_k is None and ks[0] != qs[0]:
         raise ValueError("k needs as many rows as q, or cu_k")
-    _kv8_call(q, "hxq_attn_prompt", *_view(q), *_view(k), *_view(v), dtype_code(q.dtype), _ptr(cu_q),
-              _ptr(cu_k), cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1],
-              q.shape[2], float(scale), int(causal), *_view(out), _stream(q))
+    _call_on(dev, "hxq_attn_prompt", q.data_ptr(), *_steps(qs, qt), k.data_ptr(), *_steps(ks, kt),
+             v.data_ptr(), *_steps(ks, vt), dtype_code(dt), cu_q.data_ptr(), _ptr(cu_k),
+             cu_q.numel() - 1, qs[0], ks[0], qs[1], ks[1], qs[2], scale, causal, out.data_ptr(),
+             *_steps(qs, ot), _stream(q))
     return out
+
+
+def _steps(shape, stride):
+    """Row and head stride; one that no element needs counts as 0."""
+    return stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
 
 
 def kv8_desc(k, v, k_scale, v_scale, k_tail, v_tail, blocks):
@@ -895,55 +903,63 @@ def kv8_desc(k, v, k_scale, v_scale, k_tail, v_tail, blocks):
 
 def kv8_append(q, k, v, cu_rows, cached, pos, theta, desc, q_out, k_out, v_out):
     """Rows of packed prompts into the cache (hxq_kv8_append).  q may be None with q_out None."""
-    dev = _need_heads_of(k=k, v=v) if q is None else _need_heads_of(q=q, k=k, v=v)
-    _need_i32(cu_rows=cu_rows, cached=cached, pos=pos)
-    if _need_device(cu_rows, cached, pos, q_out, k_out, v_out) != dev:
-        raise RuntimeError("tensors on different devices")
-    rows, n_kv, D = k.shape
-    if (v.shape != k.shape or n_kv != desc.n_kv_heads or D != desc.head_dim
-            or (q is not None and (q.shape[0] != rows or q.shape[2] != D))):
+    dev, ks, dt, kt, vt = k.get_device(), k.shape, k.dtype, k.stride(), v.stride()
+    qs, qt = (ks, kt) if q is None else (q.shape, q.stride())
+    if not (len(qs) == len(ks) == 3 and qt[2] == kt[2] == vt[-1] == 1 and v.get_device() == dev >= 0
+            and (q is None or q.get_device() == dev) and _flat(cu_rows, dev) and _flat(cached, dev)
+            and _flat(pos, dev) and _flat(q_out, dev) and _flat(k_out, dev) and _flat(v_out, dev)):
+        _why(dev, (("k", k), ("v", v)) if q is None else (("q", q), ("k", k), ("v", v)),
+             (("cu_rows", cu_rows), ("cached", cached), ("pos", pos), ("q_out", q_out),
+              ("k_out", k_out), ("v_out", v_out)))
+    if v.shape != ks or ks[1] != desc.n_kv_heads or ks[2] != desc.head_dim or qs[0] != ks[0] or (
+            qs[2] != ks[2]):
         raise ValueError("q must be [rows, heads, D], k and v [rows, kv heads, D] of the cache")
-    if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype):
+    if dt != v.dtype or (q is not None and q.dtype != dt):
         raise RuntimeError("q, k and v must have one dtype")
-    if cu_rows.shape != (desc.batch + 1,) or cached.shape != (desc.batch,) or (
-            pos is not None and pos.shape != (desc.batch,)):
+    _need_i32(cu_rows=cu_rows, cached=cached, pos=pos)
+    batch = desc.batch
+    if cu_rows.shape != (batch + 1,) or cached.shape != (batch,) or (
+            pos is not None and pos.shape != cached.shape):
         raise ValueError("cu_rows must be [batch + 1], cached and pos [batch]")
-    for t, like in ((q_out, q), (k_out, k), (v_out, v)):
-        if t is not None and (like is None or t.shape != like.shape
-                              or dtype_code(t.dtype) != desc.dtype):
+    for t, like in ((q_out, qs if q is not None else None), (k_out, ks), (v_out, ks)):
+        if t is not None and (t.shape != like or _DTYPE_CODE.get(t.dtype) != desc.dtype):
             raise ValueError("outputs must have the rows' shapes and the cache's 16-bit dtype")
-    heads = n_kv if q is None else q.shape[1]
-    _kv8_call(k, "hxq_kv8_append", *((None, 0, 0) if q is None else _view(q)), *_view(k), *_view(v),
-              dtype_code(k.dtype), _ptr(cu_rows), rows, heads, _ptr(cached), _ptr(pos),
-              float(theta), ctypes.byref(desc), _ptr(q_out), _ptr(k_out), _ptr(v_out), _stream(k))
+    _call_on(dev, "hxq_kv8_append", _ptr(q), *_steps(qs, qt), k.data_ptr(), *_steps(ks, kt),
+             v.data_ptr(), *_steps(ks, vt), dtype_code(dt), cu_rows.data_ptr(), ks[0], qs[1],
+             cached.data_ptr(), _ptr(pos), theta, ctypes.addressof(desc), _ptr(q_out), _ptr(k_out),
+             _ptr(v_out), _stream(k))
 
 
 def kv8_attn_decode(q, k, v, cached, pos, theta, scale, desc, weight, weight_out, out):
     """One token of each sequence over its cache (hxq_kv8_attn_decode)."""
-    dev = _need_heads_of(q=q, k=k, v=v)
-    _need_i32(cached=cached, pos=pos)
-    _need_f32(weight=weight, weight_out=weight_out)
-    if _need_device(cached, pos, weight, weight_out, out) != dev:
-        raise RuntimeError("tensors on different devices")
-    batch, heads, D = q.shape
-    if (batch != desc.batch or D != desc.head_dim or v.shape != k.shape
-            or k.shape != (batch, desc.n_kv_heads, D) or out.shape != q.shape):
+    dev, qs, ks, dt = q.get_device(), q.shape, k.shape, q.dtype
+    qt, kt, vt = q.stride(), k.stride(), v.stride()
+    if not (len(qs) == len(ks) == 3 and qt[2] == kt[2] == vt[-1] == 1 and dev >= 0
+            and k.get_device() == v.get_device() == dev and _flat(cached, dev) and _flat(pos, dev)
+            and _flat(weight, dev) and _flat(weight_out, dev) and _flat(out, dev)):
+        _why(dev, (("q", q), ("k", k), ("v", v)),
+             (("cached", cached), ("pos", pos), ("weight", weight), ("weight_out", weight_out),
+              ("out", out)))
+    batch, heads, D = qs
+    n_kv, n_blocks = desc.n_kv_heads, desc.n_blocks
+    if (batch != desc.batch or D != desc.head_dim or v.shape != ks or ks != (batch, n_kv, D)
+            or out.shape != qs):
         raise ValueError("q and out must be [batch, heads, D], k and v [batch, kv heads, D] of the "
                          "cache")
-    if not q.dtype == k.dtype == v.dtype:
+    if not dt == k.dtype == v.dtype:
         raise RuntimeError("q, k and v must have one dtype")
+    _need_i32(cached=cached, pos=pos)
     if cached.shape != (batch,) or (pos is not None and pos.shape != (batch,)):
         raise ValueError("cached and pos must be [batch]")
-    each = (batch, desc.n_kv_heads, desc.n_blocks)
     for t in (weight, weight_out):
-        if t is not None and t.shape != each:
-            raise ValueError("weights must be [batch, kv heads, n_blocks]")
-    nbytes = _kv8_workspace(batch, heads, desc.n_kv_heads, D, desc.n_blocks, weight_out is not None,
-                            q.get_device())
+        if t is not None and (t.shape != (batch, n_kv, n_blocks) or t.dtype != torch.float32):
+            raise ValueError("weights must be fp32 [batch, kv heads, n_blocks]")
+    nbytes = _kv8_workspace(batch, heads, n_kv, D, n_blocks, weight_out is not None, dev)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-    _kv8_call(q, "hxq_kv8_attn_decode", *_view(q), *_view(k), *_view(v), dtype_code(q.dtype), heads,
-              _ptr(cached), _ptr(pos), float(theta), float(scale), ctypes.byref(desc), _ptr(weight),
-              _ptr(weight_out), _ptr(out), dtype_code(out.dtype), _ptr(ws), nbytes, _stream(q))
+    _call_on(dev, "hxq_kv8_attn_decode", q.data_ptr(), *_steps(qs, qt), k.data_ptr(),
+             *_steps(ks, kt), v.data_ptr(), *_steps(ks, vt), dtype_code(dt), heads,
+             cached.data_ptr(), _ptr(pos), theta, scale, ctypes.addressof(desc), _ptr(weight),
+             _ptr(weight_out), out.data_ptr(), dtype_code(out.dtype), _ptr(ws), nbytes, _stream(q))
     return out
 
 
@@ -956,17 +972,22 @@ def _kv8_workspace(batch, heads, n_kv, D, n_blocks, weights, device):
 
 def kv8_evict(weight, blocks, cached, keep, sink, recent, weight_out, blocks_out, cached_out):
     """Choose the blocks that stay (hxq_kv8_evict)."""
-    _need_device(weight, blocks, cached, weight_out, blocks_out, cached_out)
+    dev = weight.get_device()
+    if not (dev >= 0 and _flat(weight, dev) and _flat(blocks, dev) and _flat(cached, dev)
+            and _flat(weight_out, dev) and _flat(blocks_out, dev) and _flat(cached_out, dev)):
+        _why(dev, (), (("weight", weight), ("blocks", blocks), ("cached", cached),
+                       ("weight_out", weight_out), ("blocks_out", blocks_out),
+                       ("cached_out", cached_out)))
     _need_f32(weight=weight, weight_out=weight_out)
     _need_i32(blocks=blocks, cached=cached, blocks_out=blocks_out, cached_out=cached_out)
-    if weight.dim() != 3 or cached.shape != weight.shape[:1] or any(
-            t is not None and t.shape != weight.shape for t in (blocks, weight_out, blocks_out)
-    ) or cached_out.shape != cached.shape:
+    shape = weight.shape
+    if len(shape) != 3 or cached.shape != shape[:1] or cached_out.shape != shape[:1] or (
+            weight_out.shape != shape or blocks_out.shape != shape
+            or (blocks is not None and blocks.shape != shape)):
         raise ValueError("weights and blocks must be [batch, kv heads, n_blocks], cached [batch]")
-    batch, n_kv, n_blocks = weight.shape
-    _kv8_call(weight, "hxq_kv8_evict", _ptr(weight), _ptr(blocks), _ptr(cached), batch, n_kv,
-              n_blocks, int(keep), int(sink), int(recent), _ptr(weight_out), _ptr(blocks_out),
-              _ptr(cached_out), _stream(weight))
+    _call_on(dev, "hxq_kv8_evict", weight.data_ptr(), _ptr(blocks), cached.data_ptr(), *shape, keep,
+             sink, recent, weight_out.data_ptr(), blocks_out.data_ptr(), cached_out.data_ptr(),
+             _stream(weight))
 
 
 def silu_mul(gate, up, out):

@@ -31,9 +31,9 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None):
     Returns out, [rows, heads, head_dim]; rows that belong to no sequence stay as they were in a
     given out, and are undefined in a new one."""
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     return _hxq.attn_prompt(q, k, v, cu_q, cu_k, q.shape[-1] ** -0.5 if scale is None else scale,
-                            causal, out)
+                            bool(causal), out)
 
 
 def kv8_evict(weight, blocks, cached, keep, sink=0, recent=0):
