@@ -99,28 +99,45 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
     for (int i = 0; i < ND; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, keep = -INFINITY, l = 0.f;
     const int last = min(i0 + kBM, lq) - 1;                           // the block's last query
     const int n_keys = CAUSAL ? min(lk, max(last + past + 1, 0)) : lk;   // keys that it sees
     const int lim = CAUSAL ? min(iq + past, lk - 1) : lk - 1;         // the lane's last key
     const int lim_b = min(i0 + past, lk - 1);                         // the least of the block's
     const int row_k = (ql & 0x13) | (ql & 4) << 1 | (ql & 8) >> 1;    // key of the lane's row
     if (threadIdx.x < 4) odd_rows[threadIdx.x >> 1][threadIdx.x & 1] = 0u;
-    for (int j0 = 0; j0 < n_keys; j0 += kBN) {
-        const bool edge = CAUSAL && j0 + kBN - 1 > lim_b;             // some query does not see some key
-        uint32_t *odd = odd_rows[j0 / kBN & 1];
-        u32x4 kr[NL], vr[NL];
+
+    // a step's keys and values go through registers, asked for one step ahead
+    u32x4 kr[NL], vr[NL];
+    const uint32_t off_k = static_cast<uint32_t>((threadIdx.x / CPR) * a.k.row + threadIdx.x % CPR * 8) * 2;
+    const uint32_t off_v = static_cast<uint32_t>((threadIdx.x / CPR) * a.v.row + threadIdx.x % CPR * 8) * 2;
+    constexpr int RPP = kPThr / CPR;   // rows a pass
+    const auto fetch = [&](int j0) {
+        const char *kb = reinterpret_cast<const char *>(kp + j0 * a.k.row);
+        const char *vb = reinterpret_cast<const char *>(vp + j0 * a.v.row);
+        if (j0 + kBN <= lk) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int c = threadIdx.x + i * kPThr, r = j0 + c / CPR;
-            kr[i] = vr[i] = u32x4{0u, 0u, 0u, 0u};
-            if (r < lk) {
-                kr[i] = *reinterpret_cast<const u32x4 *>(kp + r * a.k.row + c % CPR * 8);
-                vr[i] = *reinterpret_cast<const u32x4 *>(vp + r * a.v.row + c % CPR * 8);
+            for (int i = 0; i < NL; ++i) {
+                kr[i] = *reinterpret_cast<const u32x4 *>(kb + i * RPP * a.k.row * 2 + off_k);
+                vr[i] = *reinterpret_cast<const u32x4 *>(vb + i * RPP * a.v.row * 2 + off_v);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                kr[i] = vr[i] = u32x4{0u, 0u, 0u, 0u};
+                if (j0 + static_cast<int>(threadIdx.x / CPR) + i * RPP < lk) {
+                    kr[i] = *reinterpret_cast<const u32x4 *>(kb + i * RPP * a.k.row * 2 + off_k);
+                    vr[i] = *reinterpret_cast<const u32x4 *>(vb + i * RPP * a.v.row * 2 + off_v);
+                }
             }
         }
-        __syncthreads();
-        if (edge) {
+    };
+    // EDGE: some query of the block does not see some key of the step
+    const auto step = [&](int j0, auto edge_c) {
+        constexpr bool EDGE = decltype(edge_c)::value;
+        uint32_t *odd = odd_rows[j0 / kBN & 1];
+        lds_barrier();
+        if constexpr (EDGE) {
             if (threadIdx.x < 2) odd_rows[(j0 / kBN & 1) ^ 1][threadIdx.x] = 0u;
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
@@ -141,7 +158,8 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
             *reinterpret_cast<u32x4 *>(sk + swz<D>(c / CPR, c % CPR)) = kr[i];
             *reinterpret_cast<u32x4 *>(sv + swz<D>(c / CPR, c % CPR)) = vr[i];
         }
-        __syncthreads();
+        lds_barrier();
+        if (j0 + kBN < n_keys) fetch(j0 + kBN);
         f32x16 s[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -156,25 +174,31 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int j = j0 + 32 * t + 16 * (r / 8) + 8 * hh + r % 8;
-                s[t][r] = j <= lim ? s[t][r] * a.scale2 : -INFINITY;
+                if (EDGE && j0 + 32 * t + 16 * (r / 8) + 8 * hh + r % 8 > lim) s[t][r] = -INFINITY;
                 mx = fmaxf(mx, s[t][r]);
             }
-        const float mn = fmaxf(m, half_max(mx));
-        const float base = mn == -INFINITY ? 0.f : mn;   // nothing seen yet: p = 0
-        const float al = __builtin_amdgcn_exp2f(m - base);
-        m = mn;
-        l *= al;
+        // The running maximum is kept while no score passes it by more than 2^8 in weight: the sums
+        // stay far from fp32's range, and the accumulators are rescaled a few times in a row only.
+        mx = half_max(mx);
+        if (__any(mx > keep)) {
+            const float mn = fmaxf(m, mx);
+            const float al = m == mn ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.scale2);   // both may be -inf
+            m = mn;
+            keep = m + 8.f / a.scale2;
+            l *= al;
 #pragma unroll
-        for (int i = 0; i < ND; ++i)
+            for (int i = 0; i < ND; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[i][r] *= al;
+                for (int r = 0; r < 16; ++r) o[i][r] *= al;
+        }
+        const float base = m == -INFINITY ? 0.f : m * a.scale2;   // nothing seen yet: p = 0
         u32x4 p[4];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
-                const float x = __builtin_amdgcn_exp2f(s[t][r] - base), y = __builtin_amdgcn_exp2f(s[t][r + 1] - base);
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale2, -base));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[t][r + 1], a.scale2, -base));
                 l += x + y;
                 p[2 * t + r / 8][r % 8 / 2] = pack16<BF16>(x, y);
             }
@@ -187,7 +211,7 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
                 const u32x2 lo = lds_tr(sv + swz<D>(r, c) + 4 * (lane & 1)), hi = lds_tr(sv + swz<D>(r + 4, c) + 4 * (lane & 1));
                 o[i] = mfma32<BF16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[x], o[i]);
             }
-        if (edge) {
+        if constexpr (EDGE) {
             for (int t = 0; t < kBN; ++t) {
                 if (!(odd[t >> 5] >> (t & 31) & 1u) || j0 + t > lim) continue;
                 const uint16_t *row = vp + (int64_t)(j0 + t) * a.v.row + 4 * hh;
@@ -201,7 +225,11 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
                     }
             }
         }
-    }
+    };
+    if (n_keys > 0) fetch(0);
+    int j0 = 0;
+    for (; j0 + kBN <= min(n_keys, lim_b + 1); j0 += kBN) step(j0, std::false_type{});
+    for (; j0 < n_keys; j0 += kBN) step(j0, std::true_type{});
     l = half_sum(l);
     if (iq >= lq) return;
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // no key seen: zeros
@@ -235,6 +263,8 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
     HXQ_REQUIRE(q && out && cu_q && (rows_k == 0 || (k && v)), "q, k, v, cu_q and out are required");
     const HeadRows qr{q, q_row_stride, q_head_stride}, kr{k, k_row_stride, k_head_stride}, vr{v, v_row_stride, v_head_stride},
         orow{out, out_row_stride, out_head_stride};
+    HXQ_REQUIRE(k_row_stride < (1 << 24) && v_row_stride < (1 << 24) && k_row_stride >= 0 && v_row_stride >= 0,
+                "row strides of k and v must be at least 0 and less than 2^24 elements");
     HXQ_REQUIRE(rows_aligned(qr, dtype) && rows_aligned(kr, dtype) && rows_aligned(vr, dtype) && rows_aligned(orow, dtype),
                 "q, k, v and out need pointers and strides that are multiples of 16 bytes");
     const int64_t tiles = rows_q / kBM + n_seqs;
