@@ -8,7 +8,7 @@ struct PromptArgs {
     void *out;
     int64_t out_row, out_head;
     const int32_t *cu_q, *cu_k;
-    int32_t n_seqs, rows_q, rows_k, n_heads, group, tiles;
+    int32_t n_seqs, rows_q, rows_k, n_heads, group;
     float scale2;   // scale * log2(e): the softmax is in powers of two
 };
 
@@ -60,30 +60,107 @@ __device__ __forceinline__ bool drop_nonfinite(uint32_t &w) {
     return lo || hi;
 }
 
+// Tile t_id of a launch: tiles are dealt by the keys they see, the most first (the long ones do not
+// come last), over all sequences.  Tile `tile` of BM queries of a sequence with `base` tiles of earlier
+// keys has level base + tile; n(level) = tiles of that level or above is searched by halving.
+template <int BM>
+__device__ __forceinline__ bool prompt_tile(const PromptArgs &a, int t_id, int &seq, int &tile) {
+    const int lane = threadIdx.x & 63;
+    const auto shape = [&](int s, int &n, int &base) {
+        n = base = 0;
+        if (s >= a.n_seqs) return;
+        const int lq = max(seq_off(a.cu_q, s + 1, a.rows_q) - seq_off(a.cu_q, s, a.rows_q), 0);
+        const int lk = max(seq_off(a.cu_k, s + 1, a.rows_k) - seq_off(a.cu_k, s, a.rows_k), 0);
+        n = (lq + BM - 1) / BM;
+        base = max(lk - lq, 0) / BM;
+    };
+    // tiles of level L or above, in every lane
+    int n0, b0;
+    shape(lane, n0, b0);
+    const auto above = [&](int L) {
+        int v = min(max(n0 + b0 - L, 0), n0);
+        for (int s = lane + 64; s - lane < a.n_seqs; s += 64) {
+            int n, b;
+            shape(s, n, b);
+            v += min(max(n + b - L, 0), n);
+        }
+        return __builtin_amdgcn_readlane(wave_scan(v), 63);
+    };
+    int lo = 0, hi = a.rows_q / BM + a.rows_k / BM + 2;   // above(lo) > t_id >= above(hi)
+    if (t_id >= above(0)) return false;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (above(mid) > t_id) lo = mid;
+        else hi = mid;
+    }
+    // the sequences that have a tile of level lo, in order
+    const auto count = [&](int s) {
+        int n, b;
+        shape(s, n, b);
+        return lo >= b && lo < b + n ? 1 : 0;
+    };
+    int in;
+    if (!seq_tile(a.n_seqs, t_id - above(lo + 1), count, seq, in)) return false;
+    int n, b;
+    shape(seq, n, b);
+    tile = lo - b;
+    return true;
+}
+
+// V^T as an operand: keys 16 x + 8 hh + 0..7 of column 32 i + lane % 32.
+template <int D>
+__device__ __forceinline__ u32x4 v_operand(const uint16_t *v, int x, int i, int lane) {
+    const int r = 16 * x + 8 * (lane >> 5) + (lane >> 2 & 3), c = 4 * i + 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+    const u32x2 lo = lds_tr(v + swz<D>(r, c) + 4 * (lane & 1)), hi = lds_tr(v + swz<D>(r + 4, c) + 4 * (lane & 1));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// Adds what is not finite in a row of v (which was staged as 0).
+template <bool BF16, int ND>
+__device__ __forceinline__ void add_odd(const uint16_t *row, bool seen, f32x16 (&o)[ND]) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const uint16_t w = row[32 * i + 2 * (r & 12) + (r & 3)];
+            const float x = BF16 ? bf16_to_f32(w) : f16_to_f32(w);
+            o[i][r] += seen && !(fabsf(x) < INFINITY) ? x : 0.f;
+        }
+}
+
+template <bool BF16, int ND>
+__device__ __forceinline__ void store_rows(const f32x16 (&o)[ND], float sum, uint16_t *to) {
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;   // no key seen: zeros
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+            *reinterpret_cast<u32x2 *>(to + 32 * i + 2 * r) =
+                u32x2{pack16<BF16>(o[i][r] * inv, o[i][r + 1] * inv), pack16<BF16>(o[i][r + 2] * inv, o[i][r + 3] * inv)};
+}
+
 // One block: 128 query rows of one head, a wave 32 of them; steps of 64 keys with the running
 // maximum and sum of the softmax.  Both products are transposed, S^T = K Q^T and O^T = V^T P^T, so
 // that a lane holds scores of one query (its column): the softmax is in the lane but for one
 // exchange of halves, and P^T is the second product's operand in the lane's own registers.  For
 // that, row 8 a + 4 h + c of a K tile is given the key 16 (a / 2) + 8 h + 4 (a % 2) + c.
 // A weight of 0 does not undo an infinity or NaN of v: in the steps where some query of the block
-// does not see some key, such values are staged as 0, their rows marked, and added to the queries
-// that see them.
+// does not see some key, such values are staged as 0, their rows marked, and added at the end to the
+// queries that see them.
 template <bool BF16, int D, bool CAUSAL>
 __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs a) {
-    constexpr int NK = D / 16, ND = D / 32, CPR = D / 8, NL = kBN * CPR / kPThr;
+    constexpr int NK = D / 16, ND = D / 32, CPR = D / 8, NL = kBN * CPR / kPThr, RPP = kPThr / CPR;
+    constexpr int ODD = kBM / kBN + 2;   // steps in which some query does not see some key, at most
     __shared__ __attribute__((aligned(16))) uint16_t sk[kBN * D], sv[kBN * D];
-    __shared__ uint32_t odd_rows[2][2];   // of this step and the next: a bit for each key
-    const int head = blockIdx.x % a.n_heads, t_id = a.tiles - 1 - blockIdx.x / a.n_heads;
+    __shared__ uint32_t odd[ODD][2];     // a bit for each of their keys
+    const int head = blockIdx.x % a.n_heads, t_id = blockIdx.x / a.n_heads;
     int seq, tile;
-    const auto count = [&](int s) {
-        return (max(seq_off(a.cu_q, s + 1, a.rows_q) - seq_off(a.cu_q, s, a.rows_q), 0) + kBM - 1) / kBM;
-    };
-    if (!seq_tile(a.n_seqs, t_id, count, seq, tile)) return;
+    if (!prompt_tile<kBM>(a, t_id, seq, tile)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & 31, hh = lane >> 5;
     const int q_beg = seq_off(a.cu_q, seq, a.rows_q), lq = seq_off(a.cu_q, seq + 1, a.rows_q) - q_beg;
     const int k_beg = seq_off(a.cu_k, seq, a.rows_k), lk = max(seq_off(a.cu_k, seq + 1, a.rows_k) - k_beg, 0);
-    const int i0 = tile * kBM, iw = i0 + wave * 32, iq = iw + ql;   // in the sequence
+    const int i0 = tile * kBM, iq = i0 + wave * 32 + ql;   // in the sequence
     const int past = lk - lq;
     const int64_t kvh = head / a.group;
     const uint16_t *kp = static_cast<const uint16_t *>(a.k.p) + kvh * a.k.head + (int64_t)k_beg * a.k.row;
@@ -94,54 +171,53 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
 #pragma unroll
         for (int s = 0; s < NK; ++s) q[s] = *reinterpret_cast<const u32x4 *>(p + 16 * s);
     }
+    const int last = min(i0 + kBM, lq) - 1;                              // the block's last query
+    const int n_keys = CAUSAL ? min(lk, max(last + past + 1, 0)) : lk;   // keys that it sees
+    const int lim = CAUSAL ? min(iq + past, lk - 1) : lk - 1;            // the lane's last key
+    const int lim_w = CAUSAL ? min(i0 + wave * 32 + 31 + past, lk - 1) : lk - 1;   // the most of the wave's
+    const int lim_b = CAUSAL ? min(i0 + past, lk - 1) : lk - 1;          // the least of the block's
+    const int steps = (n_keys + kBN - 1) / kBN, clean = max(min(n_keys, lim_b + 1), 0) / kBN;
+    const int row_k = (ql & 0x13) | (ql & 4) << 1 | (ql & 8) >> 1;       // key of the lane's row
+    if (threadIdx.x < 2 * ODD) odd[threadIdx.x >> 1][threadIdx.x & 1] = 0u;
+
+    // a step's keys and values go through registers, asked for one step ahead
+    u32x4 kr[NL], vr[NL];
+    const int tr = threadIdx.x / CPR, tc = threadIdx.x % CPR;
+    const uint32_t off_k = static_cast<uint32_t>(tr * a.k.row + tc * 8) * 2;
+    const uint32_t off_v = static_cast<uint32_t>(tr * a.v.row + tc * 8) * 2;
+    const auto fetch = [&](int t) {
+        const char *kb = reinterpret_cast<const char *>(kp + t * kBN * a.k.row);
+        const char *vb = reinterpret_cast<const char *>(vp + t * kBN * a.v.row);
+        if ((t + 1) * kBN <= lk) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                kr[i] = *reinterpret_cast<const u32x4 *>(kb + i * RPP * a.k.row * 2 + off_k);
+                vr[i] = *reinterpret_cast<const u32x4 *>(vb + i * RPP * a.v.row * 2 + off_v);
+            }
+        } else {   // rows behind the last are the last again: no query sees them
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int64_t r = min(tr + i * RPP, lk - 1 - t * kBN);
+                kr[i] = *reinterpret_cast<const u32x4 *>(kb + (r * a.k.row + tc * 8) * 2);
+                vr[i] = *reinterpret_cast<const u32x4 *>(vb + (r * a.v.row + tc * 8) * 2);
+            }
+        }
+    };
+
     f32x16 o[ND];
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
     float m = -INFINITY, keep = -INFINITY, l = 0.f;
-    const int last = min(i0 + kBM, lq) - 1;                           // the block's last query
-    const int n_keys = CAUSAL ? min(lk, max(last + past + 1, 0)) : lk;   // keys that it sees
-    const int lim = CAUSAL ? min(iq + past, lk - 1) : lk - 1;         // the lane's last key
-    const int lim_b = min(i0 + past, lk - 1);                         // the least of the block's
-    const int row_k = (ql & 0x13) | (ql & 4) << 1 | (ql & 8) >> 1;    // key of the lane's row
-    if (threadIdx.x < 4) odd_rows[threadIdx.x >> 1][threadIdx.x & 1] = 0u;
-
-    // a step's keys and values go through registers, asked for one step ahead
-    u32x4 kr[NL], vr[NL];
-    const uint32_t off_k = static_cast<uint32_t>((threadIdx.x / CPR) * a.k.row + threadIdx.x % CPR * 8) * 2;
-    const uint32_t off_v = static_cast<uint32_t>((threadIdx.x / CPR) * a.v.row + threadIdx.x % CPR * 8) * 2;
-    constexpr int RPP = kPThr / CPR;   // rows a pass
-    const auto fetch = [&](int j0) {
-        const char *kb = reinterpret_cast<const char *>(kp + j0 * a.k.row);
-        const char *vb = reinterpret_cast<const char *>(vp + j0 * a.v.row);
-        if (j0 + kBN <= lk) {
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                kr[i] = *reinterpret_cast<const u32x4 *>(kb + i * RPP * a.k.row * 2 + off_k);
-                vr[i] = *reinterpret_cast<const u32x4 *>(vb + i * RPP * a.v.row * 2 + off_v);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                kr[i] = vr[i] = u32x4{0u, 0u, 0u, 0u};
-                if (j0 + static_cast<int>(threadIdx.x / CPR) + i * RPP < lk) {
-                    kr[i] = *reinterpret_cast<const u32x4 *>(kb + i * RPP * a.k.row * 2 + off_k);
-                    vr[i] = *reinterpret_cast<const u32x4 *>(vb + i * RPP * a.v.row * 2 + off_v);
-                }
-            }
-        }
-    };
     // EDGE: some query of the block does not see some key of the step
-    const auto step = [&](int j0, auto edge_c) {
+    const auto step = [&](int t, auto edge_c) {
         constexpr bool EDGE = decltype(edge_c)::value;
-        uint32_t *odd = odd_rows[j0 / kBN & 1];
         lds_barrier();
         if constexpr (EDGE) {
-            if (threadIdx.x < 2) odd_rows[(j0 / kBN & 1) ^ 1][threadIdx.x] = 0u;
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
-                const int r = (threadIdx.x + i * kPThr) / CPR;
+                const int r = tr + i * RPP;
                 bool found = false;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -149,33 +225,45 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
                     found |= drop_nonfinite<BF16>(w);
                     vr[i][e] = w;
                 }
-                if (found) atomicOr(&odd[r >> 5], 1u << (r & 31));
+                if (found) atomicOr(&odd[t - clean][r >> 5], 1u << (r & 31));
             }
         }
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int c = threadIdx.x + i * kPThr;
-            *reinterpret_cast<u32x4 *>(sk + swz<D>(c / CPR, c % CPR)) = kr[i];
-            *reinterpret_cast<u32x4 *>(sv + swz<D>(c / CPR, c % CPR)) = vr[i];
+            *reinterpret_cast<u32x4 *>(sk + swz<D>(tr + i * RPP, tc)) = kr[i];
+            *reinterpret_cast<u32x4 *>(sv + swz<D>(tr + i * RPP, tc)) = vr[i];
         }
         lds_barrier();
-        if (j0 + kBN < n_keys) fetch(j0 + kBN);
+        if (t + 1 < steps) fetch(t + 1);
+        if (EDGE && t * kBN > lim_w) return;   // nothing that the wave's queries see
         f32x16 s[2];
+        // the wave that multiplies goes before the one that is in its softmax
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+            for (int r = 0; r < 16; ++r) s[h][r] = 0.f;
 #pragma unroll
-            for (int x = 0; x < NK; ++x)
-                s[t] = mfma32<BF16>(*reinterpret_cast<const u32x4 *>(sk + swz<D>(32 * t + row_k, 2 * x + hh)), q[x], s[t]);
+        for (int x = 0; x < NK; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                s[h] = mfma32<BF16>(*reinterpret_cast<const u32x4 *>(sk + swz<D>(32 * h + row_k, 2 * x + hh)), q[x], s[h]);
+        // operands are read four products ahead
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int x = 0; x < 2 * NK - 4; ++x) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        __builtin_amdgcn_s_setprio(0);
         float mx = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                if (EDGE && j0 + 32 * t + 16 * (r / 8) + 8 * hh + r % 8 > lim) s[t][r] = -INFINITY;
-                mx = fmaxf(mx, s[t][r]);
+                if (EDGE && t * kBN + 32 * h + 16 * (r / 8) + 8 * hh + r % 8 > lim) s[h][r] = -INFINITY;
+                mx = fmaxf(mx, s[h][r]);
             }
         // The running maximum is kept while no score passes it by more than 2^8 in weight: the sums
         // stay far from fp32's range, and the accumulators are rescaled a few times in a row only.
@@ -194,52 +282,42 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
         const float base = m == -INFINITY ? 0.f : m * a.scale2;   // nothing seen yet: p = 0
         u32x4 p[4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale2, -base));
-                const float y = __builtin_amdgcn_exp2f(fmaf(s[t][r + 1], a.scale2, -base));
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[h][r], a.scale2, -base));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[h][r + 1], a.scale2, -base));
                 l += x + y;
-                p[2 * t + r / 8][r % 8 / 2] = pack16<BF16>(x, y);
+                p[2 * h + r / 8][r % 8 / 2] = pack16<BF16>(x, y);
             }
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
-            for (int i = 0; i < ND; ++i) {
-                // keys 16 x + 8 hh + 0..7 of column 32 i + ql
-                const int r = 16 * x + 8 * hh + (lane >> 2 & 3), c = 4 * i + 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
-                const u32x2 lo = lds_tr(sv + swz<D>(r, c) + 4 * (lane & 1)), hi = lds_tr(sv + swz<D>(r + 4, c) + 4 * (lane & 1));
-                o[i] = mfma32<BF16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[x], o[i]);
-            }
-        if constexpr (EDGE) {
-            for (int t = 0; t < kBN; ++t) {
-                if (!(odd[t >> 5] >> (t & 31) & 1u) || j0 + t > lim) continue;
-                const uint16_t *row = vp + (int64_t)(j0 + t) * a.v.row + 4 * hh;
+            for (int i = 0; i < ND; ++i) o[i] = mfma32<BF16>(v_operand<D>(sv, x, i, lane), p[x], o[i]);
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 1);
+        __builtin_amdgcn_sched_group_barrier(0x002, 36, 1);
 #pragma unroll
-                for (int i = 0; i < ND; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float x = BF16 ? bf16_to_f32(row[32 * i + 2 * (r & 12) + (r & 3)])
-                                             : f16_to_f32(row[32 * i + 2 * (r & 12) + (r & 3)]);
-                        if (!(fabsf(x) < INFINITY)) o[i][r] += x;
-                    }
-            }
+        for (int x = 0; x < 4 * ND; ++x) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+            __builtin_amdgcn_sched_group_barrier(0x002, 7, 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
         }
     };
-    if (n_keys > 0) fetch(0);
-    int j0 = 0;
-    for (; j0 + kBN <= min(n_keys, lim_b + 1); j0 += kBN) step(j0, std::false_type{});
-    for (; j0 < n_keys; j0 += kBN) step(j0, std::true_type{});
+    if (steps > 0) fetch(0);
+    int t = 0;
+    for (; t < clean; ++t) step(t, std::false_type{});
+    for (; t < steps; ++t) step(t, std::true_type{});
+
+    __syncthreads();
+    for (int t = clean; t < steps; ++t) {
+        uint64_t bits = odd[t - clean][0] | static_cast<uint64_t>(odd[t - clean][1]) << 32;
+        for (; bits; bits &= bits - 1) {
+            const int j = t * kBN + __builtin_ctzll(bits);
+            add_odd<BF16, ND>(vp + (int64_t)j * a.v.row + 4 * hh, j <= lim, o);
+        }
+    }
     l = half_sum(l);
-    if (iq >= lq) return;
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // no key seen: zeros
-    uint16_t *op = static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)(q_beg + iq) * a.out_row;
-#pragma unroll
-    for (int i = 0; i < ND; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4)
-            *reinterpret_cast<u32x2 *>(op + 32 * i + 2 * r + 4 * hh) =
-                u32x2{pack16<BF16>(o[i][r] * inv, o[i][r + 1] * inv), pack16<BF16>(o[i][r + 2] * inv, o[i][r + 3] * inv)};
+    if (iq < lq) store_rows<BF16, ND>(o, l, static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)(q_beg + iq) * a.out_row + 4 * hh);
 }
 
 }  // namespace hxq
@@ -271,7 +349,7 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
     HXQ_REQUIRE(tiles * n_heads < (int64_t{1} << 31), "too many rows");
     const PromptArgs a{qr, kr, vr, out, out_row_stride, out_head_stride, cu_q, cu_k ? cu_k : cu_q, n_seqs,
                        static_cast<int32_t>(rows_q), static_cast<int32_t>(rows_k), n_heads, n_heads / n_kv_heads,
-                       static_cast<int32_t>(tiles), scale * 1.44269504088896340736f};
+                       scale * 1.44269504088896340736f};
     const dim3 grid(static_cast<uint32_t>(tiles * n_heads));
     const auto go = [&](auto bf, auto dd) {
         constexpr bool B = decltype(bf)::value;

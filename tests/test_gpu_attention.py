@@ -66,6 +66,17 @@ def test_prompt(dev, dt, heads, kv, D, lens):
 
 
 @pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dt,D", [(BF, 128), (FP, 64), (BF, 64)])
+@pytest.mark.parametrize("lens,past", [([257], [0]), ([300, 1, 130, 0, 64], [0, 90, 63, 0, 640]),
+                                       ([512, 20], [-100, 1]), ([260, 60], [-270, -5])])
+def test_prompt_with_many_heads(dev, dt, D, lens, past, causal):
+    """Many heads over ragged sequences, keys before and fewer keys than queries."""
+    q, k, v, cu, cu_k = _prompt_case(lens, 256, 8, D, dt, 10, [max(p, -n) for p, n in zip(past, lens)])
+    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu_k.to(dev), causal=causal)
+    _check_prompt(got, q, k, v, cu, cu_k, causal=causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("lens,past", [([1, 1, 5], [0, 700, 64]), ([130, 64, 1], [31, 0, 128]),
                                        ([40, 0, 3], [-40, 17, -2]), ([257], [-200])])
 def test_prompt_continues(dev, lens, past, causal):
@@ -103,8 +114,9 @@ def test_prompt_scores_that_grow(dev):
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("lens", [[200], [70, 130]])
-def test_prompt_unseen_values_have_no_influence(dev, bad, lens):
-    q, k, v, cu, _ = _prompt_case(lens, 4, 2, 128, BF, 6)
+@pytest.mark.parametrize("heads", [4, 512])
+def test_prompt_unseen_values_have_no_influence(dev, bad, lens, heads):
+    q, k, v, cu, _ = _prompt_case(lens, heads, 2, 128, BF, 6)
     for t in (3, 40, 64, 101, 127, 199):
         v[t, 0, 5] = bad
         k[t, 1, 9] = math.nan
