@@ -36,6 +36,19 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None):
                             bool(causal), out)
 
 
+def rope_rows(q, k, v, cu_rows, pos, theta, dtype=torch.bfloat16, outs=None):
+    """Rows of packed prompts rotated to positions pos[s], pos[s] + 1, ... (q and k; v is only
+    rounded), in a 16-bit dtype: what ``HelixKV8Cache.append`` does, without a cache.  outs: three
+    tensors (or None) to write to, rows of a 16-bit cache for instance.  Returns (q, k, v)."""
+    if outs is None:
+        outs = tuple(None if t is None else torch.empty(t.shape, dtype=dtype, device=t.device)
+                     for t in (q, k, v))
+    desc = _hxq.HxqKv8(None, None, None, None, None, None, None, _hxq.dtype_code(dtype),
+                       cu_rows.numel() - 1, k.shape[1], k.shape[2], 0)
+    _hxq.kv8_append(q, k, v, cu_rows, pos, None, theta, desc, *outs)
+    return outs
+
+
 def kv8_evict(weight, blocks, cached, keep, sink=0, recent=0):
     """The blocks that stay when every sequence and kv head keeps at most `keep` full blocks: the
     first `sink`, the last `recent`, and the greatest weight between them.  Returns new (blocks,

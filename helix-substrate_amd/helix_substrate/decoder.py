@@ -10,6 +10,11 @@ greedy argmax -- are small HIP kernels (``hxq_decode.hip``).  The token id and
 position live in device memory and the argmax kernel advances them, so one
 captured HIP graph per step replays the whole generation with no host sync.
 
+A prompt goes through the layers in one pass (``prefill_prompt``: prefill GEMMs, packed causal
+attention) or token by token (``prefill``).  With ``kv_cache="e4m3"`` keys and values are held in
+8 bits (``attention.HelixKV8Cache``), for caches past the 16-bit path's 16384 tokens, and
+``evict`` cuts them to the blocks that the attention uses most.
+
 Math: transformers' Qwen2 (``models/qwen2/modeling_qwen2.py``); the residual
 stream is kept in fp32, activations entering the GEMVs are bf16.
 """
@@ -21,6 +26,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _hxq, synth
+from .attention import HelixKV8Cache, attn_prompt, rope_rows
 from .helix_linear import HelixLinear
 
 
@@ -36,6 +42,8 @@ class DecoderConfig:
     rope_theta: float = 1e6
     rms_eps: float = 1e-6
     max_seq: int = 512
+    kv_cache: str = "bf16"        # or "e4m3": 8-bit blocks of 64 tokens
+    kv_weight: bool = False       # e4m3: sum each block's attention weight, which evict() needs
 
 
 QWEN25_3B = DecoderConfig(hidden=2048, n_layers=36, n_heads=16, n_kv_heads=2, head_dim=128,
@@ -119,8 +127,21 @@ class HelixDecoder:
         self.tok = torch.zeros(1, dtype=torch.int32, device=dev)
         self.pos = torch.zeros(1, dtype=torch.int32, device=dev)
         self._argmax_ws = torch.empty(2048, dtype=torch.uint8, device=dev)
-        self.kc = [torch.zeros(c.max_seq, c.n_kv_heads, D, **bf) for _ in self.layers]
-        self.vc = [torch.zeros(c.max_seq, c.n_kv_heads, D, **bf) for _ in self.layers]
+        if c.kv_cache not in ("bf16", "e4m3"):
+            raise ValueError(f"kv_cache must be 'bf16' or 'e4m3' (got {c.kv_cache!r})")
+        self.kv8 = None
+        if c.kv_cache == "e4m3":
+            self.kc = self.vc = []
+            self.kv8 = [HelixKV8Cache.empty(1, c.n_kv_heads, D, c.max_seq, device=dev)
+                        for _ in self.layers]
+            self.kv_weight = [x.new_weight() if c.kv_weight else None for x in self.kv8]
+            self.cached = torch.zeros(1, dtype=torch.int32, device=dev)   # pos, less what was evicted
+            rows = self.qkv.view(1, -1, D)
+            self._qkv_rows = (rows[:, :c.n_heads], rows[:, c.n_heads:c.n_heads + c.n_kv_heads],
+                              rows[:, c.n_heads + c.n_kv_heads:])
+        else:
+            self.kc = [torch.zeros(c.max_seq, c.n_kv_heads, D, **bf) for _ in self.layers]
+            self.vc = [torch.zeros(c.max_seq, c.n_kv_heads, D, **bf) for _ in self.layers]
         self._qkv_mats = [_mats([L["q"], L["k"], L["v"]]) for L in self.layers]
         self._gu_mats = [_mats([L["gate"], L["up"]]) for L in self.layers]
         self._down_mats = [_mats([L["down"]]) for L in self.layers]
@@ -147,8 +168,14 @@ class HelixDecoder:
             # r = xa + delta -> xb; h = norm(r) -> q/k/v
             _hxq.gemv_multi_rmsnorm(xa, delta, L["in_norm"], c.rms_eps, xb, self._qkv_mats[li],
                                     self._group, outs=self._qkv_outs)
-            _hxq.attn_rope_decode(self.qkv, self.pos, c.n_heads, c.n_kv_heads, c.head_dim,
-                                  c.rope_theta, self.kc[li], self.vc[li], self.attn)
+            if self.kv8:
+                w = self.kv_weight[li]
+                self.kv8[li].attend(*self._qkv_rows, self.cached, pos=self.pos, theta=c.rope_theta,
+                                    weight=w, weight_out=w,
+                                    out=self.attn.view(1, c.n_heads, c.head_dim))
+            else:
+                _hxq.attn_rope_decode(self.qkv, self.pos, c.n_heads, c.n_kv_heads, c.head_dim,
+                                      c.rope_theta, self.kc[li], self.vc[li], self.attn)
             Lo = L["o"]
             _hxq.gemv(self.attn, Lo.indices, Lo._kcb, Lo.group_scale, Lo.group_offset,
                       Lo.group_size, Lo._sc_row_ptr, Lo._sc_col, Lo._sc_delta, Lo.bias,
@@ -167,9 +194,13 @@ class HelixDecoder:
         _hxq.add_rmsnorm(xa, delta, self.final_norm, c.rms_eps, self.h)
         _hxq.dense_gemv_bf16(self.embed, self.h, self.logits)
         _hxq.argmax(self.logits, self.tok, self.pos, self._argmax_ws)
+        if self.kv8:
+            self.cached.add_(1)
 
     def _step_launches_unfused(self):
         c = self.cfg
+        if self.kv8:
+            raise ValueError("the unfused step reads a bf16 cache")
         self.x.copy_(self.embed.index_select(0, self.tok.long()))
         delta = None
         for li, L in enumerate(self.layers):
@@ -199,6 +230,11 @@ class HelixDecoder:
         for t in self.kc + self.vc:
             t.zero_()
         self.pos.zero_()
+        if self.kv8:      # blocks behind the count are never read
+            self.cached.zero_()
+            for w in self.kv_weight:
+                if w is not None:
+                    w.zero_()
 
     def prefill(self, prompt_ids):
         """Feed the prompt token by token (teacher forced); leaves the greedy
@@ -209,6 +245,76 @@ class HelixDecoder:
         for t in range(ids.numel()):
             self.tok.copy_(ids[t:t + 1])
             self._step_launches()
+
+    def prefill_prompt(self, prompt_ids, chunk=4096):
+        """The prompt in one pass through the layers (pieces of at most `chunk` tokens), behind what
+        the caches hold; leaves the greedy successor of its last token in self.tok, as ``prefill``.
+        Activations between the projections are bf16 (``prefill`` keeps q, k, v and the MLP's in
+        fp32), the residual stream fp32."""
+        ids = torch.as_tensor(prompt_ids, dtype=torch.int64).to(self.device).view(-1)
+        if ids.numel() == 0:
+            raise ValueError("the prompt is empty")
+        if chunk < 1:
+            raise ValueError("chunk must be positive")
+        if int(ids.min()) < 0 or int(ids.max()) >= self.cfg.vocab:
+            raise ValueError("token id outside the vocabulary")
+        pos, cached = int(self.pos.item()), self._cached()
+        if cached + ids.numel() > self.cfg.max_seq:
+            raise ValueError("prompt longer than max_seq")
+        for t in range(0, ids.numel(), chunk):
+            piece = ids[t:t + chunk]
+            self._prompt_piece(piece, pos, cached)
+            pos += piece.numel()
+            cached += piece.numel()
+
+    def _cached(self):
+        return int((self.cached if self.kv8 else self.pos).item())
+
+    def _prompt_piece(self, ids, pos, cached):
+        c, T, dev = self.cfg, ids.numel(), self.device
+        D, nh = c.head_dim, c.n_heads
+        cu_q = torch.tensor([0, T], dtype=torch.int32, device=dev)
+        cu_k = torch.tensor([0, cached + T], dtype=torch.int32, device=dev)
+        at = torch.tensor([pos], dtype=torch.int32, device=dev)
+        x = self.embed.index_select(0, ids).float()
+        h = torch.empty(T, c.hidden, dtype=torch.bfloat16, device=dev)
+        act = torch.empty(T, c.intermediate, dtype=torch.bfloat16, device=dev)
+        delta = None
+        for li, L in enumerate(self.layers):
+            _hxq.add_rmsnorm(x, delta, L["in_norm"], c.rms_eps, h)
+            q, k, v = (L[n](h).view(T, -1, D) for n in "qkv")
+            if self.kv8:
+                before = self.kv8[li].read(0, cached) if cached else None
+                q, k, v = self.kv8[li].append(q, k, v, self.cached, cu_q, pos=at, theta=c.rope_theta)
+                if before:
+                    k, v = torch.cat([before[0], k]), torch.cat([before[1], v])
+            else:
+                kc, vc = self.kc[li], self.vc[li]
+                q = rope_rows(q, k, v, cu_q, at, c.rope_theta,
+                              outs=(torch.empty_like(q), kc[pos:pos + T], vc[pos:pos + T]))[0]
+                k, v = kc[:pos + T], vc[:pos + T]
+            a = attn_prompt(q, k, v, cu_q, cu_k)
+            _hxq.add_rmsnorm(x, L["o"](a.view(T, nh * D)), L["post_norm"], c.rms_eps, h)
+            _hxq.silu_mul(L["gate"](h).float(), L["up"](h).float(), act)
+            delta = L["down"](act)
+        _hxq.add_rmsnorm(x[-1:], delta[-1:], self.final_norm, c.rms_eps, self.h)
+        _hxq.dense_gemv_bf16(self.embed, self.h, self.logits)
+        self.pos.add_(T - 1)
+        _hxq.argmax(self.logits, self.tok, self.pos, self._argmax_ws)
+        if self.kv8:
+            self.cached.add_(T)
+
+    def evict(self, keep, sink=1, recent=4):
+        """Cut every layer's and kv head's cache to `keep` full blocks of 64 tokens: the first `sink`,
+        the last `recent`, and between them those that got the most attention weight from the tokens
+        decoded since they were stored (``kv_weight``; a prompt's own attention is not counted).
+        Positions go on as before."""
+        if not self.kv8 or self.kv_weight[0] is None:
+            raise ValueError("evict needs kv_cache='e4m3' and kv_weight=True")
+        new = None
+        for cache, w in zip(self.kv8, self.kv_weight):
+            new = cache.evict(w, self.cached, keep, sink, recent)
+        self.cached.copy_(new)
 
     def capture(self):
         """Capture one decode step in a HIP graph (weights and buffers fixed)."""
@@ -225,7 +331,7 @@ class HelixDecoder:
         """Greedy-decode n_new tokens after prefill; returns their ids (device
         int32 [n_new]).  Each step replays the captured graph; the only host
         synchronisation is the final copy."""
-        if int(self.pos.item()) + n_new > self.cfg.max_seq:
+        if self._cached() + n_new > self.cfg.max_seq:
             raise ValueError("generation would exceed max_seq")
         out = torch.empty(n_new, dtype=torch.int32, device=self.device)
         for t in range(n_new):
@@ -243,6 +349,8 @@ class HelixDecoder:
         same math as _step_launches.  Shares this decoder's buffers (token,
         position, caches, logits)."""
         c = self.cfg
+        if self.kv8:
+            raise ValueError("the one-launch step reads a bf16 cache")
         n = len(self.layers)
         arr = (_hxq.HxqDecoderLayer * n)()
         for i, L in enumerate(self.layers):
