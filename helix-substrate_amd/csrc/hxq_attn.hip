@@ -12,9 +12,7 @@ struct PromptArgs {
     float scale2;   // scale * log2(e): the softmax is in powers of two
 };
 
-constexpr int kBM = 128;    // query rows of a block
 constexpr int kBN = 64;     // keys of a step
-constexpr int kPThr = 256;
 
 template <bool BF16>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -147,20 +145,24 @@ __device__ __forceinline__ void store_rows(const f32x16 (&o)[ND], float sum, uin
 // A weight of 0 does not undo an infinity or NaN of v: in the steps where some query of the block
 // does not see some key, such values are staged as 0, their rows marked, and added at the end to the
 // queries that see them.
-template <bool BF16, int D, bool CAUSAL>
-__global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs a) {
-    constexpr int NK = D / 16, ND = D / 32, CPR = D / 8, NL = kBN * CPR / kPThr, RPP = kPThr / CPR;
-    constexpr int ODD = kBM / kBN + 2;   // steps in which some query does not see some key, at most
-    __shared__ __attribute__((aligned(16))) uint16_t sk[kBN * D], sv[kBN * D];
+//
+// NW = 4: 128 queries, one buffer, two blocks (at head_dim 64 three) on a compute unit.  NW = 8: 256
+// queries, two buffers and one barrier a step; half the bytes a query are staged.
+template <int NW, bool BF16, int D, bool CAUSAL>
+__global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArgs a) {
+    constexpr int THR = 64 * NW, BM = 32 * NW, NB = NW == 8 ? 2 : 1;
+    constexpr int NK = D / 16, ND = D / 32, CPR = D / 8, NL = kBN * CPR / THR, RPP = THR / CPR;
+    constexpr int ODD = BM / kBN + 3;    // steps in which some query does not see some key, at most
+    __shared__ __attribute__((aligned(16))) uint16_t sk[NB][kBN * D], sv[NB][kBN * D];
     __shared__ uint32_t odd[ODD][2];     // a bit for each of their keys
     const int head = blockIdx.x % a.n_heads, t_id = blockIdx.x / a.n_heads;
     int seq, tile;
-    if (!prompt_tile<kBM>(a, t_id, seq, tile)) return;
+    if (!prompt_tile<BM>(a, t_id, seq, tile)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & 31, hh = lane >> 5;
     const int q_beg = seq_off(a.cu_q, seq, a.rows_q), lq = seq_off(a.cu_q, seq + 1, a.rows_q) - q_beg;
     const int k_beg = seq_off(a.cu_k, seq, a.rows_k), lk = max(seq_off(a.cu_k, seq + 1, a.rows_k) - k_beg, 0);
-    const int i0 = tile * kBM, iq = i0 + wave * 32 + ql;   // in the sequence
+    const int i0 = tile * BM, iq = i0 + wave * 32 + ql;   // in the sequence
     const int past = lk - lq;
     const int64_t kvh = head / a.group;
     const uint16_t *kp = static_cast<const uint16_t *>(a.k.p) + kvh * a.k.head + (int64_t)k_beg * a.k.row;
@@ -171,12 +173,12 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
 #pragma unroll
         for (int s = 0; s < NK; ++s) q[s] = *reinterpret_cast<const u32x4 *>(p + 16 * s);
     }
-    const int last = min(i0 + kBM, lq) - 1;                              // the block's last query
+    const int last = min(i0 + BM, lq) - 1;                              // the block's last query
     const int n_keys = CAUSAL ? min(lk, max(last + past + 1, 0)) : lk;   // keys that it sees
     const int lim = CAUSAL ? min(iq + past, lk - 1) : lk - 1;            // the lane's last key
     const int lim_w = CAUSAL ? min(i0 + wave * 32 + 31 + past, lk - 1) : lk - 1;   // the most of the wave's
     const int lim_b = CAUSAL ? min(i0 + past, lk - 1) : lk - 1;          // the least of the block's
-    const int steps = (n_keys + kBN - 1) / kBN, clean = max(min(n_keys, lim_b + 1), 0) / kBN;
+    const int steps = (n_keys + kBN - 1) / kBN, clean = max(min(n_keys, lim_b + 1), 0) / kBN & -NB;
     const int row_k = (ql & 0x13) | (ql & 4) << 1 | (ql & 8) >> 1;       // key of the lane's row
     if (threadIdx.x < 2 * ODD) odd[threadIdx.x >> 1][threadIdx.x & 1] = 0u;
 
@@ -210,11 +212,8 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
     float m = -INFINITY, keep = -INFINITY, l = 0.f;
-    // EDGE: some query of the block does not see some key of the step
-    const auto step = [&](int t, auto edge_c) {
-        constexpr bool EDGE = decltype(edge_c)::value;
-        lds_barrier();
-        if constexpr (EDGE) {
+    const auto put = [&](int t, int b) {
+        if (t >= clean) {
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const int r = tr + i * RPP;
@@ -230,11 +229,14 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
         }
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            *reinterpret_cast<u32x4 *>(sk + swz<D>(tr + i * RPP, tc)) = kr[i];
-            *reinterpret_cast<u32x4 *>(sv + swz<D>(tr + i * RPP, tc)) = vr[i];
+            *reinterpret_cast<u32x4 *>(sk[b] + swz<D>(tr + i * RPP, tc)) = kr[i];
+            *reinterpret_cast<u32x4 *>(sv[b] + swz<D>(tr + i * RPP, tc)) = vr[i];
         }
-        lds_barrier();
-        if (t + 1 < steps) fetch(t + 1);
+    };
+    // EDGE: some query of the block does not see some key of the step
+    const auto compute = [&](int t, auto b_c, auto edge_c) {
+        constexpr bool EDGE = decltype(edge_c)::value;
+        const uint16_t *k = sk[decltype(b_c)::value], *v = sv[decltype(b_c)::value];
         if (EDGE && t * kBN > lim_w) return;   // nothing that the wave's queries see
         f32x16 s[2];
         // the wave that multiplies goes before the one that is in its softmax
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
         for (int x = 0; x < NK; ++x)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                s[h] = mfma32<BF16>(*reinterpret_cast<const u32x4 *>(sk + swz<D>(32 * h + row_k, 2 * x + hh)), q[x], s[h]);
+                s[h] = mfma32<BF16>(*reinterpret_cast<const u32x4 *>(k + swz<D>(32 * h + row_k, 2 * x + hh)), q[x], s[h]);
         // operands are read four products ahead
         __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
@@ -293,7 +295,7 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
-            for (int i = 0; i < ND; ++i) o[i] = mfma32<BF16>(v_operand<D>(sv, x, i, lane), p[x], o[i]);
+            for (int i = 0; i < ND; ++i) o[i] = mfma32<BF16>(v_operand<D>(v, x, i, lane), p[x], o[i]);
         __builtin_amdgcn_sched_group_barrier(0x100, 6, 1);
         __builtin_amdgcn_sched_group_barrier(0x002, 36, 1);
 #pragma unroll
@@ -303,10 +305,38 @@ __global__ __launch_bounds__(kPThr, 2) void attn_prompt_kernel(const PromptArgs 
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
         }
     };
-    if (steps > 0) fetch(0);
+    const auto step = [&](int t, auto b_c, auto edge_c) {
+        if constexpr (NB == 1) {
+            lds_barrier();
+            put(t, 0);
+            lds_barrier();
+        }
+        if (t + 1 < steps) fetch(t + 1);
+        compute(t, b_c, edge_c);
+        if constexpr (NB == 2) {
+            if (t + 1 < steps) put(t + 1, decltype(b_c)::value ^ 1);
+            lds_barrier();
+        }
+    };
+    if (steps > 0) {
+        fetch(0);
+        if constexpr (NB == 2) {
+            lds_barrier();   // odd[] is cleared
+            put(0, 0);
+            lds_barrier();
+        }
+    }
+    using B0 = std::integral_constant<int, 0>;
+    using B1 = std::integral_constant<int, NB - 1>;
     int t = 0;
-    for (; t < clean; ++t) step(t, std::false_type{});
-    for (; t < steps; ++t) step(t, std::true_type{});
+    for (; t < clean; t += NB) {
+        step(t, B0{}, std::false_type{});
+        if constexpr (NB == 2) step(t + 1, B1{}, std::false_type{});
+    }
+    for (; t < steps; t += NB) {
+        step(t, B0{}, std::true_type{});
+        if (NB == 2 && t + 1 < steps) step(t + 1, B1{}, std::true_type{});
+    }
 
     __syncthreads();
     for (int t = clean; t < steps; ++t) {
@@ -334,8 +364,8 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
     HXQ_REQUIRE(attn_dtype(dtype, false), "q, k and v must be bf16 or fp16");
     HXQ_REQUIRE(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128");
     HXQ_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads");
-    HXQ_REQUIRE(n_seqs >= 0 && rows_q >= 0 && rows_k >= 0 && rows_q < (int64_t{1} << 31) - 4 * kBM &&
-                    rows_k < (int64_t{1} << 31) - 4 * kBM, "bad sizes");
+    HXQ_REQUIRE(n_seqs >= 0 && rows_q >= 0 && rows_k >= 0 && rows_q < (int64_t{1} << 31) - 1024 &&
+                    rows_k < (int64_t{1} << 31) - 1024, "bad sizes");
     HXQ_REQUIRE(scale == scale && scale > 0.f && scale < INFINITY, "scale must be positive and finite");
     if (n_seqs == 0 || rows_q == 0) return HXQ_OK;
     HXQ_REQUIRE(q && out && cu_q && (rows_k == 0 || (k && v)), "q, k, v, cu_q and out are required");
@@ -345,7 +375,11 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
                 "row strides of k and v must be at least 0 and less than 2^24 elements");
     HXQ_REQUIRE(rows_aligned(qr, dtype) && rows_aligned(kr, dtype) && rows_aligned(vr, dtype) && rows_aligned(orow, dtype),
                 "q, k, v and out need pointers and strides that are multiples of 16 bytes");
-    const int64_t tiles = rows_q / kBM + n_seqs;
+    // 8 waves where their blocks still go twice over the compute units (one document of 16384 tokens, 16
+    // heads: 990 us against 1085; twelve sequences of 200 to 2048, 28 heads: 249 against 248); below that 4
+    // fill more of them (211 tokens, 16 heads: 13 us against 17).
+    const int nw = head_dim == 128 && rows_q / 256 * n_heads >= 2 * device_cu_count() ? 8 : 4;
+    const int64_t tiles = rows_q / (32 * nw) + n_seqs;
     HXQ_REQUIRE(tiles * n_heads < (int64_t{1} << 31), "too many rows");
     const PromptArgs a{qr, kr, vr, out, out_row_stride, out_head_stride, cu_q, cu_k ? cu_k : cu_q, n_seqs,
                        static_cast<int32_t>(rows_q), static_cast<int32_t>(rows_k), n_heads, n_heads / n_kv_heads,
@@ -354,8 +388,15 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
     const auto go = [&](auto bf, auto dd) {
         constexpr bool B = decltype(bf)::value;
         constexpr int D = decltype(dd)::value;
-        if (causal) hipLaunchKernelGGL((attn_prompt_kernel<B, D, true>), grid, dim3(kPThr), 0, stream, a);
-        else hipLaunchKernelGGL((attn_prompt_kernel<B, D, false>), grid, dim3(kPThr), 0, stream, a);
+        const auto by_nw = [&](auto w) {
+            constexpr int NW = decltype(w)::value;
+            if (causal) hipLaunchKernelGGL((attn_prompt_kernel<NW, B, D, true>), grid, dim3(64 * NW), 0, stream, a);
+            else hipLaunchKernelGGL((attn_prompt_kernel<NW, B, D, false>), grid, dim3(64 * NW), 0, stream, a);
+        };
+        if constexpr (D == 128) {
+            if (nw == 8) return by_nw(std::integral_constant<int, 8>{});
+        }
+        by_nw(std::integral_constant<int, 4>{});
     };
     const auto by_d = [&](auto bf) {
         if (head_dim == 128) go(bf, std::integral_constant<int, 128>{});

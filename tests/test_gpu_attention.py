@@ -66,12 +66,12 @@ def test_prompt(dev, dt, heads, kv, D, lens):
 
 
 @pytest.mark.parametrize("causal", [True, False])
-@pytest.mark.parametrize("dt,D", [(BF, 128), (FP, 64), (BF, 64)])
+@pytest.mark.parametrize("dt,D", [(BF, 128), (FP, 128), (BF, 64)])
 @pytest.mark.parametrize("lens,past", [([257], [0]), ([300, 1, 130, 0, 64], [0, 90, 63, 0, 640]),
                                        ([512, 20], [-100, 1]), ([260, 60], [-270, -5])])
 def test_prompt_with_many_heads(dev, dt, D, lens, past, causal):
     """Many heads over ragged sequences, keys before and fewer keys than queries."""
-    q, k, v, cu, cu_k = _prompt_case(lens, 256, 8, D, dt, 10, [max(p, -n) for p, n in zip(past, lens)])
+    q, k, v, cu, cu_k = _prompt_case(lens, 512, 8, D, dt, 10, [max(p, -n) for p, n in zip(past, lens)])
     got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu_k.to(dev), causal=causal)
     _check_prompt(got, q, k, v, cu, cu_k, causal=causal)
 
@@ -116,11 +116,14 @@ def test_prompt_scores_that_grow(dev):
 @pytest.mark.parametrize("lens", [[200], [70, 130]])
 @pytest.mark.parametrize("heads", [4, 512])
 def test_prompt_unseen_values_have_no_influence(dev, bad, lens, heads):
+    """512 heads: with the rows behind the sequences enough for the 8-wave blocks."""
     q, k, v, cu, _ = _prompt_case(lens, heads, 2, 128, BF, 6)
+    if heads == 512:
+        q = torch.cat([q, torch.zeros(100, heads, 128, dtype=BF)])
     for t in (3, 40, 64, 101, 127, 199):
         v[t, 0, 5] = bad
         k[t, 1, 9] = math.nan
-    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev))[:, :2]
+    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu.to(dev))[:, :2]
     # kv head 0 (heads 0, 1): NaN or infinities in v reach exactly the queries that see them
     h0 = got.cpu().double()
     for s in range(len(lens)):
