@@ -58,51 +58,69 @@ __device__ __forceinline__ bool drop_nonfinite(uint32_t &w) {
     return lo || hi;
 }
 
+// A block's part of a packed batch.
+struct PromptTile {
+    int tile, q_beg, lq, k_beg, lk;   // tile of its sequence; the sequence's rows
+};
+
 // Tile t_id of a launch: tiles are dealt by the keys they see, the most first (the long ones do not
 // come last), over all sequences.  Tile `tile` of BM queries of a sequence with `base` tiles of earlier
-// keys has level base + tile; n(level) = tiles of that level or above is searched by halving.
+// keys has level base + tile; the number of tiles of a level or above is searched by halving.  The
+// first 64 sequences are held one in a lane: one round of loads, then registers only.
 template <int BM>
-__device__ __forceinline__ bool prompt_tile(const PromptArgs &a, int t_id, int &seq, int &tile) {
+__device__ __forceinline__ bool prompt_tile(const PromptArgs &a, int t_id, PromptTile &at) {
     const int lane = threadIdx.x & 63;
-    const auto shape = [&](int s, int &n, int &base) {
-        n = base = 0;
-        if (s >= a.n_seqs) return;
-        const int lq = max(seq_off(a.cu_q, s + 1, a.rows_q) - seq_off(a.cu_q, s, a.rows_q), 0);
-        const int lk = max(seq_off(a.cu_k, s + 1, a.rows_k) - seq_off(a.cu_k, s, a.rows_k), 0);
-        n = (lq + BM - 1) / BM;
-        base = max(lk - lq, 0) / BM;
+    struct Seq {
+        int q_beg, lq, k_beg, lk, n, base;
     };
-    // tiles of level L or above, in every lane
-    int n0, b0;
-    shape(lane, n0, b0);
+    const auto load = [&](int s) {
+        Seq x{0, 0, 0, 0, 0, 0};
+        if (s >= a.n_seqs) return x;
+        x.q_beg = seq_off(a.cu_q, s, a.rows_q);
+        x.lq = max(seq_off(a.cu_q, s + 1, a.rows_q) - x.q_beg, 0);
+        x.k_beg = seq_off(a.cu_k, s, a.rows_k);
+        x.lk = max(seq_off(a.cu_k, s + 1, a.rows_k) - x.k_beg, 0);
+        x.n = (x.lq + BM - 1) / BM;
+        x.base = max(x.lk - x.lq, 0) / BM;
+        return x;
+    };
+    const auto of_level = [](const Seq &x, int L) { return min(max(x.n + x.base - L, 0), x.n); };   // L or above
+    const Seq first = load(lane);
     const auto above = [&](int L) {
-        int v = min(max(n0 + b0 - L, 0), n0);
-        for (int s = lane + 64; s - lane < a.n_seqs; s += 64) {
-            int n, b;
-            shape(s, n, b);
-            v += min(max(n + b - L, 0), n);
-        }
+        int v = of_level(first, L);
+        for (int s = lane + 64; s - lane < a.n_seqs; s += 64) v += of_level(load(s), L);
         return __builtin_amdgcn_readlane(wave_scan(v), 63);
     };
-    int lo = 0, hi = a.rows_q / BM + a.rows_k / BM + 2;   // above(lo) > t_id >= above(hi)
     if (t_id >= above(0)) return false;
+    int lo = 0, hi = first.n + first.base;   // above(lo) > t_id >= above(hi)
+    if (a.n_seqs > 64) hi = a.rows_q / BM + a.rows_k / BM + 2;
+    else {
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) hi = max(hi, __shfl_xor(hi, m, kWave));
+    }
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
         if (above(mid) > t_id) lo = mid;
         else hi = mid;
     }
-    // the sequences that have a tile of level lo, in order
-    const auto count = [&](int s) {
-        int n, b;
-        shape(s, n, b);
-        return lo >= b && lo < b + n ? 1 : 0;
-    };
-    int in;
-    if (!seq_tile(a.n_seqs, t_id - above(lo + 1), count, seq, in)) return false;
-    int n, b;
-    shape(seq, n, b);
-    tile = lo - b;
-    return true;
+    // among the sequences that have a tile of level lo, in order
+    int left = t_id - above(lo + 1);
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+        const Seq x = s0 ? load(s0 + lane) : first;
+        const uint64_t has = __ballot(lo >= x.base && lo < x.base + x.n);
+        const int c = __builtin_popcountll(has);
+        if (left < c) {
+            // the lane with `left` others before it
+            const int mine = __builtin_popcountll(has & ((1ull << lane) - 1));
+            const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot((has >> lane & 1) && mine == left)));
+            at = PromptTile{lo - __builtin_amdgcn_readlane(x.base, l), __builtin_amdgcn_readlane(x.q_beg, l),
+                            __builtin_amdgcn_readlane(x.lq, l), __builtin_amdgcn_readlane(x.k_beg, l),
+                            __builtin_amdgcn_readlane(x.lk, l)};
+            return true;
+        }
+        left -= c;
+    }
+    return false;
 }
 
 // V^T as an operand: keys 16 x + 8 hh + 0..7 of column 32 i + lane % 32.
@@ -155,16 +173,21 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
     constexpr int ODD = BM / kBN + 3;    // steps in which some query does not see some key, at most
     __shared__ __attribute__((aligned(16))) uint16_t sk[NB][kBN * D], sv[NB][kBN * D];
     __shared__ uint32_t odd[ODD][2];     // a bit for each of their keys
-    const int head = blockIdx.x % a.n_heads, t_id = blockIdx.x / a.n_heads;
-    int seq, tile;
-    if (!prompt_tile<BM>(a, t_id, seq, tile)) return;
+    // Blocks go round the 8 dies.  The heads of one kv head and tile stay on a die, and with them the
+    // tiles of a kv head on as few as there are: their keys and values come from its L2 (28 heads over
+    // 4, twelve sequences: 82 % of the requests instead of 49).
+    const int n_kv = a.n_heads / a.group, die = blockIdx.x % 8, turn = blockIdx.x / 8, row = turn / a.group;
+    int unit = row * 8 + die;
+    // 8 dies hold 8 / n_kv tiles a row, the most work first: every other row goes the other way round
+    if (row & 1 && 8 % n_kv == 0) unit += 8 - n_kv - 2 * (die / n_kv * n_kv);
+    const int kvh = unit % n_kv, head = kvh * a.group + turn % a.group;
+    PromptTile at;
+    if (!prompt_tile<BM>(a, unit / n_kv, at)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & 31, hh = lane >> 5;
-    const int q_beg = seq_off(a.cu_q, seq, a.rows_q), lq = seq_off(a.cu_q, seq + 1, a.rows_q) - q_beg;
-    const int k_beg = seq_off(a.cu_k, seq, a.rows_k), lk = max(seq_off(a.cu_k, seq + 1, a.rows_k) - k_beg, 0);
-    const int i0 = tile * BM, iq = i0 + wave * 32 + ql;   // in the sequence
+    const int q_beg = at.q_beg, lq = at.lq, k_beg = at.k_beg, lk = at.lk;
+    const int i0 = at.tile * BM, iq = i0 + wave * 32 + ql;   // in the sequence
     const int past = lk - lq;
-    const int64_t kvh = head / a.group;
     const uint16_t *kp = static_cast<const uint16_t *>(a.k.p) + kvh * a.k.head + (int64_t)k_beg * a.k.row;
     const uint16_t *vp = static_cast<const uint16_t *>(a.v.p) + kvh * a.v.head + (int64_t)k_beg * a.v.row;
     u32x4 q[NK];
@@ -380,11 +403,12 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
     // fill more of them (211 tokens, 16 heads: 13 us against 17).
     const int nw = head_dim == 128 && rows_q / 256 * n_heads >= 2 * device_cu_count() ? 8 : 4;
     const int64_t tiles = rows_q / (32 * nw) + n_seqs;
-    HXQ_REQUIRE(tiles * n_heads < (int64_t{1} << 31), "too many rows");
+    const int64_t blocks = (tiles * n_kv_heads + 7) / 8 * 8 * (n_heads / n_kv_heads);
+    HXQ_REQUIRE(blocks < (int64_t{1} << 31), "too many rows");
     const PromptArgs a{qr, kr, vr, out, out_row_stride, out_head_stride, cu_q, cu_k ? cu_k : cu_q, n_seqs,
                        static_cast<int32_t>(rows_q), static_cast<int32_t>(rows_k), n_heads, n_heads / n_kv_heads,
                        scale * 1.44269504088896340736f};
-    const dim3 grid(static_cast<uint32_t>(tiles * n_heads));
+    const dim3 grid(static_cast<uint32_t>(blocks));
     const auto go = [&](auto bf, auto dd) {
         constexpr bool B = decltype(bf)::value;
         constexpr int D = decltype(dd)::value;
