@@ -287,7 +287,7 @@ struct DecodeArgs {
     const int32_t *cached, *pos;
     RopeTable rope;
     float scale2;                    // scale * log2(e): the softmax is in powers of two
-    int32_t out_dtype, n_heads, splits;
+    int32_t out_dtype, n_heads, splits, group, htiles;
     hxq_kv8 c;
     const float *w_in;
     float *w_out;
@@ -364,8 +364,13 @@ __global__ __launch_bounds__(kDThr, 1) void kv8_decode_kernel(const DecodeArgs a
     __shared__ float cs[HALF], sn[HALF];
     __shared__ __attribute__((aligned(16))) float so[NW][kHT][D];
     __shared__ float sm[NW][kHT], sl[NW][kHT], red[NW];
-    const int n_kv = a.c.n_kv_heads, group = a.n_heads / n_kv, htiles = (group + kHT - 1) / kHT;
-    const int ht = blockIdx.y % htiles, kvh = blockIdx.y / htiles % n_kv, b = blockIdx.y / htiles / n_kv;
+    // Everything that the first loads need in one round of scalar loads: left to itself each value is
+    // fetched where it is used, and eight round trips come before the first byte of the cache.
+    asm volatile("" ::"s"(a.cached), "s"(a.pos), "s"(a.q.p), "s"(a.q.row), "s"(a.q.head), "s"(a.k.p), "s"(a.k.row), "s"(a.k.head),
+                 "s"(a.v.p), "s"(a.v.row), "s"(a.v.head), "s"(a.c.k), "s"(a.c.v), "s"(a.c.k_scale), "s"(a.c.v_scale),
+                 "s"(a.c.blocks), "s"(a.c.n_blocks), "s"(a.c.n_kv_heads), "s"(a.n_heads), "s"(a.group), "s"(a.htiles), "s"(a.splits));
+    const int n_kv = a.c.n_kv_heads, group = a.group, htiles = a.htiles;
+    const int ht = blockIdx.y % htiles, kvh = blockIdx.y / htiles, b = blockIdx.z;
     const int h0 = kvh * group + ht * kHT, nh = min(kHT, group - ht * kHT);
     // the new token's values are asked for first: they are needed first, and loads return in order
     float x1[NP], x2[NP], xv = 0.f;
@@ -377,7 +382,7 @@ __global__ __launch_bounds__(kDThr, 1) void kv8_decode_kernel(const DecodeArgs a
         x1[i] = load_act<DT>(p, at);
         x2[i] = load_act<DT>(p, at + HALF);
     }
-    if (threadIdx.x < D) xv = load_act<DT>(a.v.p, b * a.v.row + kvh * a.v.head + threadIdx.x);
+    xv = load_act<DT>(a.v.p, b * a.v.row + kvh * a.v.head + threadIdx.x % D);
     const int cached = a.cached[b];
     if (cached < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -419,11 +424,11 @@ __global__ __launch_bounds__(kDThr, 1) void kv8_decode_kernel(const DecodeArgs a
 #pragma unroll
         for (int i = 0; i < NT; ++i) vr[i] = vp[(16 * i + lh) * 4 + kq];
     };
-    if (u0 + wave < uf) {
-        find(u0 + wave);
-        load_k();
-        load_v();
-    }
+    // Every wave asks, also one that has no unit (for a block that another reads): with loads behind a
+    // branch the wait for the token's values, asked for before, would be for all of them.
+    find(max(min(u0 + wave, uf - 1), 0));
+    load_k();
+    load_v();
 
     // the new token: rotation in fp32, q in three bf16 (24 bits)
     const bool rope = a.rope.on;
@@ -969,14 +974,15 @@ extern "C" int hxq_kv8_attn_decode(const void *q, int64_t q_row_stride, int64_t 
     HXQ_REQUIRE(theta >= 0.f && theta < INFINITY && scale == scale && fabsf(scale) < INFINITY, "theta and scale must be finite");
     HXQ_REQUIRE(weight_out || !weight_in, "weight_in without weight_out");
     const int64_t tiles = kv8_tiles(cache->batch, n_heads, cache->n_kv_heads);
-    HXQ_REQUIRE(tiles <= 65535 && (int64_t)cache->batch * n_heads < (int64_t{1} << 31), "batch * heads too large");
+    HXQ_REQUIRE(cache->batch <= 65535 && tiles / cache->batch <= 65535 && (int64_t)cache->batch * n_heads < (int64_t{1} << 31), "batch or heads too large");
     const int splits = kv8_splits(tiles, cache->n_blocks);
     const Kv8Ws w = kv8_ws(cache->batch, n_heads, splits, cache->head_dim, cache->n_blocks, weight_out != nullptr);
     HXQ_REQUIRE(w.bytes == 0 || (workspace && workspace_bytes >= w.bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "workspace too small or not 16-byte aligned");
     char *ws = static_cast<char *>(workspace);
     const DecodeArgs a{{q, q_row_stride, q_head_stride}, {k, k_row_stride, k_head_stride}, {v, v_row_stride, v_head_stride},
-                       cached, pos, rope_table(theta, cache->head_dim), scale * 1.44269504088896340736f, out_dtype, n_heads, splits, *cache,
+                       cached, pos, rope_table(theta, cache->head_dim), scale * 1.44269504088896340736f, out_dtype, n_heads, splits,
+                       n_heads / cache->n_kv_heads, (n_heads / cache->n_kv_heads + kHT - 1) / kHT, *cache,
                        weight_in, weight_out, out, reinterpret_cast<float *>(ws),
                        reinterpret_cast<float2 *>(ws + w.ml), reinterpret_cast<float2 *>(ws + w.share)};
     // what the second launch has to do: rows to join, chunks of weights
@@ -984,7 +990,7 @@ extern "C" int hxq_kv8_attn_decode(const void *q, int64_t q_row_stride, int64_t 
     const int64_t chunks = weight_out ? (int64_t)cache->batch * cache->n_kv_heads * ((cache->n_blocks + kThr - 1) / kThr) : 0;
     HXQ_REQUIRE(rows + chunks < (int64_t{1} << 31), "batch * heads or blocks too large");
     const dim3 join(static_cast<uint32_t>(rows + chunks));
-    const dim3 grid(splits, static_cast<uint32_t>(tiles));
+    const dim3 grid(splits, static_cast<uint32_t>(tiles / cache->batch), cache->batch);
     const auto go = [&](auto dt, auto bf, auto dd) {
         constexpr int T = decltype(dt)::value, D = decltype(dd)::value;
         constexpr bool B = decltype(bf)::value;
