@@ -880,16 +880,26 @@ def _steps(shape, stride):
     return stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
 
 
+_KV16 = {torch.bfloat16: HXQ_BF16, torch.float16: HXQ_F16}
+
+
 def kv8_desc(k, v, k_scale, v_scale, k_tail, v_tail, blocks):
     """hxq_kv8 of a cache's tensors."""
-    _need_device(k, v, k_scale, v_scale, k_tail, v_tail, blocks)
+    dev, i32 = k.get_device(), torch.int32
+    if not (dev >= 0 and k.is_contiguous() and _flat(v, dev) and _flat(k_scale, dev)
+            and _flat(v_scale, dev) and _flat(k_tail, dev) and _flat(v_tail, dev)
+            and _flat(blocks, dev)):
+        _why(dev, (), (("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale),
+                       ("k_tail", k_tail), ("v_tail", v_tail), ("blocks", blocks)))
     batch, n_kv, n_blocks, block, D = k.shape
+    dt = _KV16.get(k_tail.dtype)
     if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
         raise RuntimeError("k and v must be float8_e4m3fn")
-    if k_tail.dtype not in (torch.bfloat16, torch.float16) or v_tail.dtype != k_tail.dtype:
+    if dt is None or v_tail.dtype != k_tail.dtype:
         raise RuntimeError("k_tail and v_tail must be bfloat16 or float16, both alike")
-    _need_f32(k_scale=k_scale, v_scale=v_scale)
-    _need_i32(blocks=blocks)
+    if not (k_scale.dtype == v_scale.dtype == torch.float32
+            and (blocks is None or blocks.dtype == i32)):
+        raise RuntimeError("k_scale and v_scale must be float32, blocks int32")
     each = (batch, n_kv, n_blocks)
     if (block != KV8_BLOCK or v.shape != (*each, D, block) or k_scale.shape != each
             or v_scale.shape != each or k_tail.shape != (batch, n_kv, block, D)
@@ -897,8 +907,7 @@ def kv8_desc(k, v, k_scale, v_scale, k_tail, v_tail, blocks):
             or (blocks is not None and blocks.shape != each)):
         raise ValueError("cache shapes do not fit together")
     return HxqKv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                  k_tail.data_ptr(), v_tail.data_ptr(), _ptr(blocks), dtype_code(k_tail.dtype),
-                  batch, n_kv, D, n_blocks)
+                  k_tail.data_ptr(), v_tail.data_ptr(), _ptr(blocks), dt, batch, n_kv, D, n_blocks)
 
 
 def kv8_append(q, k, v, cu_rows, cached, pos, theta, desc, q_out, k_out, v_out):
@@ -941,25 +950,28 @@ def kv8_attn_decode(q, k, v, cached, pos, theta, scale, desc, weight, weight_out
              (("cached", cached), ("pos", pos), ("weight", weight), ("weight_out", weight_out),
               ("out", out)))
     batch, heads, D = qs
-    n_kv, n_blocks = desc.n_kv_heads, desc.n_blocks
-    if (batch != desc.batch or D != desc.head_dim or v.shape != ks or ks != (batch, n_kv, D)
-            or out.shape != qs):
+    n_kv, n_blocks = ks[1], desc.n_blocks
+    if (batch != desc.batch or D != desc.head_dim or n_kv != desc.n_kv_heads or v.shape != ks
+            or ks[0] != batch or ks[2] != D or out.shape != qs):
         raise ValueError("q and out must be [batch, heads, D], k and v [batch, kv heads, D] of the "
                          "cache")
     if not dt == k.dtype == v.dtype:
         raise RuntimeError("q, k and v must have one dtype")
-    _need_i32(cached=cached, pos=pos)
-    if cached.shape != (batch,) or (pos is not None and pos.shape != (batch,)):
-        raise ValueError("cached and pos must be [batch]")
-    for t in (weight, weight_out):
-        if t is not None and (t.shape != (batch, n_kv, n_blocks) or t.dtype != torch.float32):
-            raise ValueError("weights must be fp32 [batch, kv heads, n_blocks]")
+    if (cached.dtype != torch.int32 or cached.shape != (batch,)
+            or (pos is not None and (pos.dtype != torch.int32 or pos.shape != (batch,)))):
+        raise RuntimeError("cached and pos must be int32 [batch]")
+    if weight_out is not None or weight is not None:
+        for t in (weight, weight_out):
+            if t is not None and (t.shape != (batch, n_kv, n_blocks) or t.dtype != torch.float32):
+                raise ValueError("weights must be fp32 [batch, kv heads, n_blocks]")
+    if batch == 1 or heads == 1 or n_kv == 1:   # strides that no element needs count as 0
+        qt, kt, vt = _steps(qs, qt), _steps(ks, kt), _steps(ks, vt)
     nbytes = _kv8_workspace(batch, heads, n_kv, D, n_blocks, weight_out is not None, dev)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-    _call_on(dev, "hxq_kv8_attn_decode", q.data_ptr(), *_steps(qs, qt), k.data_ptr(),
-             *_steps(ks, kt), v.data_ptr(), *_steps(ks, vt), dtype_code(dt), heads,
-             cached.data_ptr(), _ptr(pos), theta, scale, ctypes.addressof(desc), _ptr(weight),
-             _ptr(weight_out), out.data_ptr(), dtype_code(out.dtype), _ptr(ws), nbytes, _stream(q))
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+    _call_on(dev, "hxq_kv8_attn_decode", q.data_ptr(), qt[0], qt[1], k.data_ptr(), kt[0], kt[1],
+             v.data_ptr(), vt[0], vt[1], dtype_code(dt), heads, cached.data_ptr(), _ptr(pos), theta,
+             scale, ctypes.addressof(desc), _ptr(weight), _ptr(weight_out), out.data_ptr(),
+             dtype_code(out.dtype), _ptr(ws), nbytes, _stream(q))
     return out
 
 

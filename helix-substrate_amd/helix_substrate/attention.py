@@ -54,7 +54,7 @@ def kv8_evict(weight, blocks, cached, keep, sink=0, recent=0):
     first `sink`, the last `recent`, and the greatest weight between them.  Returns new (blocks,
     weight, cached) tensors; see ``HelixKV8Cache.evict`` for a cache that is cut in place."""
     weight_out, cached_out = torch.empty_like(weight), torch.empty_like(cached)
-    blocks_out = torch.empty(weight.shape, dtype=torch.int32, device=weight.device)
+    blocks_out = torch.empty_like(weight, dtype=torch.int32)
     _hxq.kv8_evict(weight, blocks, cached, keep, sink, recent, weight_out, blocks_out, cached_out)
     return blocks_out, weight_out, cached_out
 
@@ -127,8 +127,9 @@ class HelixKV8Cache:
         cache's 16-bit dtype (q, k, v), which `attn_prompt` takes; q None gives None.  outs: three
         tensors (or None) to write them to.  Tokens past max_tokens are not stored."""
         if outs is None:
-            outs = tuple(None if t is None else torch.empty(t.shape, dtype=self.dtype, device=t.device)
-                         for t in (q, k, v))
+            dt = self.dtype
+            outs = (None if q is None else q.new_empty(q.shape, dtype=dt),
+                    k.new_empty(k.shape, dtype=dt), v.new_empty(v.shape, dtype=dt))
         _hxq.kv8_append(q, k, v, cu_rows, cached, pos, theta, self._desc, *outs)
         return outs
 
@@ -139,7 +140,7 @@ class HelixKV8Cache:
         (None: zeros) plus each block's share of the softmax summed over the query heads of its kv
         head; it may be weight.  Returns (out [batch, heads, D], weight_out)."""
         if out is None:
-            out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+            out = q.new_empty(q.shape, dtype=out_dtype)
         _hxq.kv8_attn_decode(q, k, v, cached, pos, theta,
                              q.shape[-1] ** -0.5 if scale is None else scale, self._desc, weight,
                              weight_out, out)
