@@ -398,10 +398,11 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
                 "row strides of k and v must be at least 0 and less than 2^24 elements");
     HXQ_REQUIRE(rows_aligned(qr, dtype) && rows_aligned(kr, dtype) && rows_aligned(vr, dtype) && rows_aligned(orow, dtype),
                 "q, k, v and out need pointers and strides that are multiples of 16 bytes");
-    // 8 waves where their blocks still go twice over the compute units (one document of 16384 tokens, 16
-    // heads: 990 us against 1085; twelve sequences of 200 to 2048, 28 heads: 249 against 248); below that 4
-    // fill more of them (211 tokens, 16 heads: 13 us against 17).
-    const int nw = head_dim == 128 && rows_q / 256 * n_heads >= 2 * device_cu_count() ? 8 : 4;
+    // 8 waves for long sequences whose blocks reach every compute unit, 4 for the others (16 heads over 2,
+    // us with 4 and 8 waves: one of 4096 tokens 136 and 124, of 8192 335 and 305, eight of 2048 178 and 173;
+    // sixteen of 1024 116 and 123, one of 211 13 and 17): two blocks of 4 a unit hide each other's start,
+    // 8 waves stage half the bytes.
+    const int nw = head_dim == 128 && rows_q >= int64_t{1536} * n_seqs && rows_q / 256 * n_heads >= device_cu_count() ? 8 : 4;
     const int64_t tiles = rows_q / (32 * nw) + n_seqs;
     const int64_t blocks = (tiles * n_kv_heads + 7) / 8 * 8 * (n_heads / n_kv_heads);
     HXQ_REQUIRE(blocks < (int64_t{1} << 31), "too many rows");

@@ -65,14 +65,23 @@ def test_prompt(dev, dt, heads, kv, D, lens):
     _check_prompt(got, q, k, v, cu, cu)
 
 
+def _behind(q, n_seqs):
+    """q with rows of no sequence behind it, to 1536 rows a sequence: a large call, which the 8-wave
+    blocks take (from 64 heads on)."""
+    more = torch.full((max(1536 * n_seqs - q.shape[0], 0), *q.shape[1:]), math.nan, dtype=q.dtype)
+    return torch.cat([q, more])
+
+
 @pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("large", [True, False])
 @pytest.mark.parametrize("dt,D", [(BF, 128), (FP, 128), (BF, 64)])
 @pytest.mark.parametrize("lens,past", [([257], [0]), ([300, 1, 130, 0, 64], [0, 90, 63, 0, 640]),
-                                       ([512, 20], [-100, 1]), ([260, 60], [-270, -5])])
-def test_prompt_with_many_heads(dev, dt, D, lens, past, causal):
-    """Many heads over ragged sequences, keys before and fewer keys than queries."""
-    q, k, v, cu, cu_k = _prompt_case(lens, 512, 8, D, dt, 10, [max(p, -n) for p, n in zip(past, lens)])
-    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu_k.to(dev), causal=causal)
+                                       ([512, 20], [-100, 1]), ([260, 60], [-270, -5]), ([700], [333])])
+def test_prompt_with_many_heads(dev, dt, D, lens, past, causal, large):
+    """Many heads over ragged sequences, keys before and fewer keys than queries; both block sizes."""
+    q, k, v, cu, cu_k = _prompt_case(lens, 64, 8, D, dt, 10, [max(p, -n) for p, n in zip(past, lens)])
+    got = attn_prompt((_behind(q, len(lens)) if large else q).to(dev), k.to(dev), v.to(dev), cu.to(dev),
+                      cu_k.to(dev), causal=causal)[:q.shape[0]]
     _check_prompt(got, q, k, v, cu, cu_k, causal=causal)
 
 
@@ -114,12 +123,11 @@ def test_prompt_scores_that_grow(dev):
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("lens", [[200], [70, 130]])
-@pytest.mark.parametrize("heads", [4, 512])
+@pytest.mark.parametrize("heads", [4, 64])
 def test_prompt_unseen_values_have_no_influence(dev, bad, lens, heads):
-    """512 heads: with the rows behind the sequences enough for the 8-wave blocks."""
     q, k, v, cu, _ = _prompt_case(lens, heads, 2, 128, BF, 6)
-    if heads == 512:
-        q = torch.cat([q, torch.zeros(100, heads, 128, dtype=BF)])
+    if heads == 64:
+        q = _behind(q, len(lens))
     for t in (3, 40, 64, 101, 127, 199):
         v[t, 0, 5] = bad
         k[t, 1, 9] = math.nan
@@ -132,9 +140,9 @@ def test_prompt_unseen_values_have_no_influence(dev, bad, lens, heads):
         assert torch.isfinite(h0[r.start:first]).all()
         assert torch.isfinite(h0[r, :, 6:]).all() and torch.isfinite(h0[r, :, :5]).all()
         assert not torch.isfinite(h0[first:r.stop, :, 5]).any()
-    q, k, v = q[:, :2], k[:, :1], v[:, :1].clone()
+    q, k, v = q[:200, :2], k[:, :1], v[:, :1].clone()
     v[:, 0, 5] = 0
-    got = got.clone()
+    got = got[:200].clone()
     got[..., 5] = 0
     _check_prompt(got, q, k, v, cu, cu)
 
