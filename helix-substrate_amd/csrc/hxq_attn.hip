@@ -1,4 +1,6 @@
 // Attention of packed prompts: causal, grouped heads, sequences of different lengths.
+#include <algorithm>
+
 #include "hxq_attn.h"
 
 namespace hxq {
@@ -10,7 +12,21 @@ struct PromptArgs {
     const int32_t *cu_q, *cu_k;
     int32_t n_seqs, rows_q, rows_k, n_heads, group;
     float scale2;   // scale * log2(e): the softmax is in powers of two
+    int32_t splits, by_die;
+    float *part;    // [rows_q * n_heads][splits][D]: sums of p v of a split's keys
+    float2 *ml;     // [rows_q * n_heads][splits]: their maximum (in powers of two) and sum of p
 };
+
+constexpr int kMaxSplits = 16;
+
+// Steps of 64 keys of one split; at least 4.
+__device__ __forceinline__ int steps_per_split(int steps, int splits) { return max((steps + splits - 1) / splits, 4); }
+
+// Keys that the queries up to `last` of a sequence see.
+template <bool CAUSAL>
+__device__ __forceinline__ int keys_seen(int last, int lq, int lk) {
+    return CAUSAL ? min(lk, max(last + lk - lq + 1, 0)) : lk;
+}
 
 constexpr int kBN = 64;     // keys of a step
 
@@ -166,21 +182,30 @@ __device__ __forceinline__ void store_rows(const f32x16 (&o)[ND], float sum, uin
 //
 // NW = 4: 128 queries, one buffer, two blocks (at head_dim 64 three) on a compute unit.  NW = 8: 256
 // queries, two buffers and one barrier a step; half the bytes a query are staged.
-template <int NW, bool BF16, int D, bool CAUSAL>
+// SPLIT: blockIdx.y takes a part of the keys and leaves its sums for attn_join_kernel.
+template <int NW, bool BF16, int D, bool CAUSAL, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArgs a) {
     constexpr int THR = 64 * NW, BM = 32 * NW, NB = NW == 8 ? 2 : 1;
     constexpr int NK = D / 16, ND = D / 32, CPR = D / 8, NL = kBN * CPR / THR, RPP = THR / CPR;
     constexpr int ODD = BM / kBN + 3;    // steps in which some query does not see some key, at most
     __shared__ __attribute__((aligned(16))) uint16_t sk[NB][kBN * D], sv[NB][kBN * D];
     __shared__ uint32_t odd[ODD][2];     // a bit for each of their keys
-    // Blocks go round the 8 dies.  The heads of one kv head and tile stay on a die, and with them the
-    // tiles of a kv head on as few as there are: their keys and values come from its L2 (28 heads over
-    // 4, twelve sequences: 82 % of the requests instead of 49).
-    const int n_kv = a.n_heads / a.group, die = blockIdx.x % 8, turn = blockIdx.x / 8, row = turn / a.group;
-    int unit = row * 8 + die;
-    // 8 dies hold 8 / n_kv tiles a row, the most work first: every other row goes the other way round
-    if (row & 1 && 8 % n_kv == 0) unit += 8 - n_kv - 2 * (die / n_kv * n_kv);
-    const int kvh = unit % n_kv, head = kvh * a.group + turn % a.group;
+    // Blocks go round the 8 dies.  In large calls the heads of one kv head and tile stay on a die, and with
+    // them the tiles of a kv head on as few as there are: their keys and values come from its L2 (28 heads
+    // over 4, twelve sequences: 82 % of the requests instead of 49).  8 dies hold 8 / n_kv tiles a row, the
+    // most work first: every other row goes the other way round.  In small calls the heads go round.
+    const int n_kv = a.n_heads / a.group;
+    int unit, head;
+    if (a.by_die) {
+        const int die = blockIdx.x % 8, turn = blockIdx.x / 8, row = turn / a.group;
+        unit = row * 8 + die;
+        if (row & 1 && 8 % n_kv == 0) unit += 8 - n_kv - 2 * (die / n_kv * n_kv);
+        head = unit % n_kv * a.group + turn % a.group;
+    } else {
+        head = blockIdx.x % a.n_heads;
+        unit = blockIdx.x / a.n_heads * n_kv;
+    }
+    const int kvh = head / a.group;
     PromptTile at;
     if (!prompt_tile<BM>(a, unit / n_kv, at)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -197,12 +222,19 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
         for (int s = 0; s < NK; ++s) q[s] = *reinterpret_cast<const u32x4 *>(p + 16 * s);
     }
     const int last = min(i0 + BM, lq) - 1;                              // the block's last query
-    const int n_keys = CAUSAL ? min(lk, max(last + past + 1, 0)) : lk;   // keys that it sees
+    const int n_keys = keys_seen<CAUSAL>(last, lq, lk);
     const int lim = CAUSAL ? min(iq + past, lk - 1) : lk - 1;            // the lane's last key
     const int lim_w = CAUSAL ? min(i0 + wave * 32 + 31 + past, lk - 1) : lk - 1;   // the most of the wave's
     const int lim_b = CAUSAL ? min(i0 + past, lk - 1) : lk - 1;          // the least of the block's
     const int steps = (n_keys + kBN - 1) / kBN, clean = max(min(n_keys, lim_b + 1), 0) / kBN & -NB;
     const int row_k = (ql & 0x13) | (ql & 4) << 1 | (ql & 8) >> 1;       // key of the lane's row
+    int t0 = 0, t1 = steps;
+    if constexpr (SPLIT) {
+        const int per = steps_per_split(steps, a.splits);
+        t0 = min(static_cast<int>(blockIdx.y) * per, steps);
+        t1 = min(t0 + per, steps);
+        if (t0 == t1 && t0 > 0) return;   // no part; the first is written also where nothing is seen
+    }
     if (threadIdx.x < 2 * ODD) odd[threadIdx.x >> 1][threadIdx.x & 1] = 0u;
 
     // a step's keys and values go through registers, asked for one step ahead
@@ -334,15 +366,15 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
             put(t, 0);
             lds_barrier();
         }
-        if (t + 1 < steps) fetch(t + 1);
+        if (t + 1 < t1) fetch(t + 1);
         compute(t, b_c, edge_c);
         if constexpr (NB == 2) {
-            if (t + 1 < steps) put(t + 1, decltype(b_c)::value ^ 1);
+            if (t + 1 < t1) put(t + 1, decltype(b_c)::value ^ 1);
             lds_barrier();
         }
     };
-    if (steps > 0) {
-        fetch(0);
+    if (t0 < t1) {
+        fetch(t0);
         if constexpr (NB == 2) {
             lds_barrier();   // odd[] is cleared
             put(0, 0);
@@ -351,18 +383,18 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
     }
     using B0 = std::integral_constant<int, 0>;
     using B1 = std::integral_constant<int, NB - 1>;
-    int t = 0;
-    for (; t < clean; t += NB) {
+    int t = t0;
+    for (; t < min(clean, t1); t += NB) {
         step(t, B0{}, std::false_type{});
         if constexpr (NB == 2) step(t + 1, B1{}, std::false_type{});
     }
-    for (; t < steps; t += NB) {
+    for (; t < t1; t += NB) {
         step(t, B0{}, std::true_type{});
-        if (NB == 2 && t + 1 < steps) step(t + 1, B1{}, std::true_type{});
+        if (NB == 2 && t + 1 < t1) step(t + 1, B1{}, std::true_type{});
     }
 
     __syncthreads();
-    for (int t = clean; t < steps; ++t) {
+    for (int t = max(clean, t0); t < t1; ++t) {
         uint64_t bits = odd[t - clean][0] | static_cast<uint64_t>(odd[t - clean][1]) << 32;
         for (; bits; bits &= bits - 1) {
             const int j = t * kBN + __builtin_ctzll(bits);
@@ -370,19 +402,109 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
         }
     }
     l = half_sum(l);
-    if (iq < lq) store_rows<BF16, ND>(o, l, static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)(q_beg + iq) * a.out_row + 4 * hh);
+    if (iq >= lq) return;
+    if constexpr (SPLIT) {
+        const int64_t at = ((int64_t)(q_beg + iq) * a.n_heads + head) * a.splits + blockIdx.y;
+        float *to = a.part + at * D + 4 * hh;
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+                *reinterpret_cast<f32x4 *>(to + 32 * i + 2 * r) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+        if (hh == 0) a.ml[at] = float2{m * a.scale2, l};
+    } else {
+        store_rows<BF16, ND>(o, l, static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)(q_beg + iq) * a.out_row + 4 * hh);
+    }
+}
+
+// The splits of every query joined: a wave for a query of a head (32 blocks for the 128 queries of a
+// tile of the kernel above).
+template <bool BF16, int D, bool CAUSAL>
+__global__ __launch_bounds__(256) void attn_join_kernel(const PromptArgs a) {
+    constexpr int R = D / kWave, BM = 128;
+    const int unit = blockIdx.x / 32, head = unit % a.n_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    PromptTile at;
+    if (!prompt_tile<BM>(a, unit / a.n_heads, at)) return;
+    const int last = min(at.tile * BM + BM, at.lq) - 1;
+    const int steps = (keys_seen<CAUSAL>(last, at.lq, at.lk) + kBN - 1) / kBN, per = steps_per_split(steps, a.splits);
+    const int n = max((steps + per - 1) / per, 1);
+    const int i = at.tile * BM + blockIdx.x % 32 * 4 + wave;
+    if (i > last) return;
+    const int64_t row = (int64_t)(at.q_beg + i) * a.n_heads + head;
+    const float2 e = lane < n ? a.ml[row * a.splits + lane] : float2{-INFINITY, 0.f};
+    const float *pt = a.part + row * a.splits * D + lane * R;
+    float p[kMaxSplits][R];
+#pragma unroll
+    for (int s = 0; s < kMaxSplits; ++s)
+        if (s < n)
+#pragma unroll
+            for (int r = 0; r < R; ++r) p[s][r] = pt[s * D + r];
+    float mm = e.x;
+#pragma unroll
+    for (int s = kMaxSplits / 2; s >= 1; s >>= 1) mm = fmaxf(mm, __shfl_xor(mm, s, kWave));
+    mm = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(mm)));
+    // a split of which the query sees nothing has sum 0 (and NaN where all that it sees is NaN)
+    const float f = e.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(e.x - mm);
+    const float ll = wave_sum(f * e.y);
+    const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
+    uint16_t *to = static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)(at.q_beg + i) * a.out_row + lane * R;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float x = 0.f;
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s)
+            if (s < n) x = fmaf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s)), p[s][r], x);
+        to[r] = BF16 ? f32_to_bf16(x * inv) : f32_to_f16(x * inv);
+    }
 }
 
 }  // namespace hxq
 
 using namespace hxq;
 
+namespace {
+
+struct PromptPlan {
+    int nw, splits;
+    int64_t part_bytes, bytes;   // workspace: part, then ml
+};
+
+// What depends on sizes that the host knows; lengths of sequences are on the device.
+PromptPlan prompt_plan(int64_t rows_q, int64_t rows_k, int64_t n_seqs, int64_t n_heads, int32_t D) {
+    const int64_t cus = device_cu_count();
+    PromptPlan p{4, 1, 0, 0};
+    // 8 waves for long sequences whose blocks reach every compute unit, 4 for the others (16 heads over 2,
+    // us with 4 and 8 waves: one of 4096 tokens 136 and 124, of 8192 335 and 305, eight of 2048 178 and 173;
+    // sixteen of 1024 116 and 123, one of 211 13 and 17): two blocks of 4 a unit hide each other's start,
+    // 8 waves stage half the bytes.
+    if (D == 128 && rows_q >= 1536 * n_seqs && rows_q / 256 * n_heads >= cus) p.nw = 8;
+    // Few queries over many keys: the keys are split until there are two blocks a compute unit, at least
+    // 512 keys each (16 heads, us with one block and split: 8 queries over 8000 keys 216 and 29, 512 over 8500
+    // 230 and 61, 1024 over 2048 62 and 43, a prompt of 1500 48 and 49).
+    const int64_t blocks = std::max(std::min(rows_q, n_seqs), (rows_q + 127) / 128) * n_heads;
+    if (p.nw == 4 && blocks < cus)
+        p.splits = static_cast<int>(std::max<int64_t>(1, std::min({2 * cus / blocks, rows_k / n_seqs / 512, int64_t{kMaxSplits}})));
+    if (p.splits > 1) {
+        p.part_bytes = rows_q * n_heads * p.splits * D * 4;
+        p.bytes = p.part_bytes + rows_q * n_heads * p.splits * 8;
+    }
+    return p;
+}
+
+}  // namespace
+
+extern "C" int64_t hxq_attn_prompt_workspace_bytes(int64_t rows_q, int64_t rows_k, int32_t n_seqs, int32_t n_heads,
+                                                   int32_t head_dim) {
+    if (rows_q < 0 || rows_k < 0 || n_seqs < 0 || n_heads <= 0 || (head_dim != 64 && head_dim != 128)) return -1;
+    return rows_q && n_seqs ? prompt_plan(rows_q, rows_k, n_seqs, n_heads, head_dim).bytes : 0;
+}
+
 extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
                                int64_t k_row_stride, int64_t k_head_stride, const void *v, int64_t v_row_stride,
                                int64_t v_head_stride, int32_t dtype, const int32_t *cu_q, const int32_t *cu_k,
                                int32_t n_seqs, int64_t rows_q, int64_t rows_k, int32_t n_heads, int32_t n_kv_heads,
                                int32_t head_dim, float scale, int32_t causal, void *out, int64_t out_row_stride,
-                               int64_t out_head_stride, hipStream_t stream) {
+                               int64_t out_head_stride, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
     clear_error();
     HXQ_REQUIRE(attn_dtype(dtype, false), "q, k and v must be bf16 or fp16");
     HXQ_REQUIRE(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128");
@@ -398,30 +520,39 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
                 "row strides of k and v must be at least 0 and less than 2^24 elements");
     HXQ_REQUIRE(rows_aligned(qr, dtype) && rows_aligned(kr, dtype) && rows_aligned(vr, dtype) && rows_aligned(orow, dtype),
                 "q, k, v and out need pointers and strides that are multiples of 16 bytes");
-    // 8 waves for long sequences whose blocks reach every compute unit, 4 for the others (16 heads over 2,
-    // us with 4 and 8 waves: one of 4096 tokens 136 and 124, of 8192 335 and 305, eight of 2048 178 and 173;
-    // sixteen of 1024 116 and 123, one of 211 13 and 17): two blocks of 4 a unit hide each other's start,
-    // 8 waves stage half the bytes.
-    const int nw = head_dim == 128 && rows_q >= int64_t{1536} * n_seqs && rows_q / 256 * n_heads >= device_cu_count() ? 8 : 4;
-    const int64_t tiles = rows_q / (32 * nw) + n_seqs;
-    const int64_t blocks = (tiles * n_kv_heads + 7) / 8 * 8 * (n_heads / n_kv_heads);
+    const PromptPlan plan = prompt_plan(rows_q, rows_k, n_seqs, n_heads, head_dim);
+    HXQ_REQUIRE(plan.bytes == 0 || (workspace && workspace_bytes >= plan.bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+                "workspace too small or not 16-byte aligned");
+    const int64_t tiles = rows_q / (32 * plan.nw) + n_seqs;
+    // eight tiles of a kv head a die: below that some dies would go short (8 queries, 8192 keys, 16 heads: 50
+    // us by die, 23 round)
+    const bool by_die = tiles * n_kv_heads >= 64;
+    const int64_t blocks = by_die ? (tiles * n_kv_heads + 7) / 8 * 8 * (n_heads / n_kv_heads) : tiles * n_heads;
     HXQ_REQUIRE(blocks < (int64_t{1} << 31), "too many rows");
     const PromptArgs a{qr, kr, vr, out, out_row_stride, out_head_stride, cu_q, cu_k ? cu_k : cu_q, n_seqs,
                        static_cast<int32_t>(rows_q), static_cast<int32_t>(rows_k), n_heads, n_heads / n_kv_heads,
-                       scale * 1.44269504088896340736f};
-    const dim3 grid(static_cast<uint32_t>(blocks));
+                       scale * 1.44269504088896340736f, plan.splits, by_die, static_cast<float *>(workspace),
+                       reinterpret_cast<float2 *>(static_cast<char *>(workspace) + plan.part_bytes)};
+    const dim3 grid(static_cast<uint32_t>(blocks), plan.splits), join(static_cast<uint32_t>(plan.splits > 1 ? tiles * n_heads * 32 : 0));
     const auto go = [&](auto bf, auto dd) {
         constexpr bool B = decltype(bf)::value;
         constexpr int D = decltype(dd)::value;
-        const auto by_nw = [&](auto w) {
-            constexpr int NW = decltype(w)::value;
-            if (causal) hipLaunchKernelGGL((attn_prompt_kernel<NW, B, D, true>), grid, dim3(64 * NW), 0, stream, a);
-            else hipLaunchKernelGGL((attn_prompt_kernel<NW, B, D, false>), grid, dim3(64 * NW), 0, stream, a);
+        const auto by_c = [&](auto cc) {
+            constexpr bool C = decltype(cc)::value;
+            if (plan.splits > 1) {
+                hipLaunchKernelGGL((attn_prompt_kernel<4, B, D, C, true>), grid, dim3(256), 0, stream, a);
+                hipLaunchKernelGGL((attn_join_kernel<B, D, C>), join, dim3(256), 0, stream, a);
+                return;
+            }
+            if constexpr (D == 128)
+                if (plan.nw == 8) {
+                    hipLaunchKernelGGL((attn_prompt_kernel<8, B, D, C, false>), grid, dim3(512), 0, stream, a);
+                    return;
+                }
+            hipLaunchKernelGGL((attn_prompt_kernel<4, B, D, C, false>), grid, dim3(256), 0, stream, a);
         };
-        if constexpr (D == 128) {
-            if (nw == 8) return by_nw(std::integral_constant<int, 8>{});
-        }
-        by_nw(std::integral_constant<int, 4>{});
+        if (causal) by_c(std::true_type{});
+        else by_c(std::false_type{});
     };
     const auto by_d = [&](auto bf) {
         if (head_dim == 128) go(bf, std::integral_constant<int, 128>{});

@@ -114,7 +114,7 @@ SIGNATURES = {
     "hxq_dense_gemv_bf16": [P, P, I32, I64, I64, P, P],
     "hxq_argmax": [P, I64, P, P, P, P],
     "hxq_attn_prompt": [P, I64, I64, P, I64, I64, P, I64, I64, I32, P, P, I32, I64, I64, I32, I32,
-                        I32, F32, I32, P, I64, I64, P],
+                        I32, F32, I32, P, I64, I64, P, I64, P],
     "hxq_kv8_append": [P, I64, I64, P, I64, I64, P, I64, I64, I32, P, I64, I32, P, P, F32, P, P, P,
                        P, P],
     "hxq_kv8_attn_decode": [P, I64, I64, P, I64, I64, P, I64, I64, I32, I32, P, P, F32, F32, P, P,
@@ -155,6 +155,7 @@ SIGNATURES_I64 = {
     "hxq_gemm_workspace_bytes": [I64, I64, I64],
     "hxq_gemm_noalloc_max_bytes": [],
     "hxq_prefill_gemm_workspace_bytes": [I64, I64, I64],
+    "hxq_attn_prompt_workspace_bytes": [I64, I64, I32, I32, I32],
     "hxq_kv8_attn_decode_workspace_bytes": [I32, I32, I32, I32, I32, I32],
     "hxq_prefill_gemm_plan": [I64, I64, I64, I32, I32, I32],
 }
@@ -868,11 +869,21 @@ def attn_prompt(q, k, v, cu_q, cu_k, scale, causal, out):
         raise ValueError("cu_q and cu_k must be [n_seqs + 1]")
     if cu_k is None and ks[0] != qs[0]:
         raise ValueError("k needs as many rows as q, or cu_k")
+    n_seqs, rows, rows_k, heads, D = cu_q.numel() - 1, qs[0], ks[0], qs[1], qs[2]
+    nbytes = _prompt_workspace(rows, rows_k, n_seqs, heads, D, dev)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
     _call_on(dev, "hxq_attn_prompt", q.data_ptr(), *_steps(qs, qt), k.data_ptr(), *_steps(ks, kt),
-             v.data_ptr(), *_steps(ks, vt), dtype_code(dt), cu_q.data_ptr(), _ptr(cu_k),
-             cu_q.numel() - 1, qs[0], ks[0], qs[1], ks[1], qs[2], scale, causal, out.data_ptr(),
-             *_steps(qs, ot), _stream(q))
+             v.data_ptr(), *_steps(ks, vt), dtype_code(dt), cu_q.data_ptr(), _ptr(cu_k), n_seqs,
+             rows, rows_k, heads, ks[1], D, scale, causal, out.data_ptr(), *_steps(qs, ot),
+             _ptr(ws), nbytes, _stream(q))
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _prompt_workspace(rows_q, rows_k, n_seqs, heads, D, device):
+    """hxq_attn_prompt_workspace_bytes on `device` (it counts the compute units)."""
+    with torch.cuda.device(device):
+        return lib().hxq_attn_prompt_workspace_bytes(rows_q, rows_k, n_seqs, heads, D)
 
 
 def _steps(shape, stride):

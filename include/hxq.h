@@ -543,15 +543,20 @@ int hxq_argmax(const float *logits, int64_t n, int32_t *out_id, int32_t *pos,
  * gives zeros.  Keys that a query does not see have no influence, whatever they hold.  dtype (q, k,
  * v, out): HXQ_BF16 or HXQ_F16; scores, softmax and sums are fp32, the softmax weights are rounded
  * to dtype before the product with v.  Rows of out that belong to no sequence are left as they
- * were; offsets are clamped to [0, rows_q] and [0, rows_k].
+ * were; offsets are clamped to [0, rows_q] and [0, rows_k].  Row strides of k and v: 0 to 2^24 - 1
+ * elements.  workspace: device scratch of hxq_attn_prompt_workspace_bytes(...) bytes (0 but for few
+ * queries over many keys), written and read within the call.
  */
+int64_t hxq_attn_prompt_workspace_bytes(int64_t rows_q, int64_t rows_k, int32_t n_seqs,
+                                        int32_t n_heads, int32_t head_dim);
 int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
                     int64_t k_row_stride, int64_t k_head_stride, const void *v,
                     int64_t v_row_stride, int64_t v_head_stride, int32_t dtype,
                     const int32_t *cu_q, const int32_t *cu_k, int32_t n_seqs, int64_t rows_q,
                     int64_t rows_k, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                     float scale, int32_t causal, void *out, int64_t out_row_stride,
-                    int64_t out_head_stride, hipStream_t stream);
+                    int64_t out_head_stride, void *workspace, int64_t workspace_bytes,
+                    hipStream_t stream);
 
 /*
  * The 8-bit cache: per sequence and kv head, blocks of HXQ_KV8_BLOCK = 64 tokens.

@@ -24,7 +24,8 @@ def _message(lib):
 
 PROMPT = dict(q=A, q_row=2048, q_head=128, k=A, k_row=256, k_head=128, v=A, v_row=256, v_head=128,
               dtype=_hxq.HXQ_BF16, cu_q=A, cu_k=None, n=1, rows_q=8, rows_k=8, heads=16, kv=2, D=128,
-              scale=0.1, causal=1, out=A, o_row=2048, o_head=128, stream=None)
+              scale=0.1, causal=1, out=A, o_row=2048, o_head=128, ws=None, ws_bytes=0,
+              stream=None)
 
 
 @pytest.mark.parametrize("change,text", [
@@ -34,7 +35,10 @@ PROMPT = dict(q=A, q_row=2048, q_head=128, k=A, k_row=256, k_head=128, v=A, v_ro
     (dict(o_row=2052), "16 bytes"), (dict(q=None), "required"), (dict(out=None), "required"),
     (dict(cu_q=None), "required"), (dict(k=None), "required"), (dict(n=-1), "sizes"),
     (dict(rows_q=1 << 31), "sizes"), (dict(rows_k=-1), "sizes"), (dict(scale=math.nan), "scale"),
-    (dict(scale=0.0), "scale"), (dict(scale=math.inf), "scale")])
+    (dict(scale=0.0), "scale"), (dict(scale=math.inf), "scale"),
+    (dict(k_row=1 << 24), "row strides"), (dict(v_row=-8), "row strides"),
+    (dict(rows_k=8192), "workspace"), (dict(rows_k=8192, ws=A, ws_bytes=64), "workspace"),
+    (dict(rows_k=8192, ws=A + 8, ws_bytes=1 << 40), "workspace")])
 def test_prompt_refuses(lib, change, text):
     assert lib.hxq_attn_prompt(*{**PROMPT, **change}.values()) == 1
     assert text in _message(lib)
@@ -43,6 +47,15 @@ def test_prompt_refuses(lib, change, text):
 def test_prompt_of_nothing(lib):
     assert lib.hxq_attn_prompt(*{**PROMPT, "n": 0}.values()) == 0
     assert lib.hxq_attn_prompt(*{**PROMPT, "rows_q": 0, "q": None}.values()) == 0
+
+
+def test_prompt_workspace(lib):
+    need = lib.hxq_attn_prompt_workspace_bytes
+    assert need(8, 8, 1, 16, 128) == 0 and need(4096, 4096, 1, 16, 128) == 0
+    assert need(0, 8, 1, 16, 128) == 0 and need(8, 8, 0, 16, 128) == 0
+    assert need(8, 8, 1, 16, 96) == -1 and need(-1, 8, 1, 16, 128) == -1
+    rest, bytes_a_split = divmod(need(8, 8192, 1, 16, 128), 8 * 16 * (128 * 4 + 8))
+    assert rest > 1 and bytes_a_split == 0
 
 
 def _desc(**change):

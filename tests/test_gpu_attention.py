@@ -97,6 +97,30 @@ def test_prompt_continues(dev, lens, past, causal):
         assert (got[:200] == 0).all()
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dt,heads,kv,D", [(BF, 16, 2, 128), (FP, 4, 4, 64)])
+@pytest.mark.parametrize("lens,past", [([1], [5000]), ([3, 130], [2000, 1500]), ([5, 0, 60, 70], [9, 6000, -30, 8190]),
+                                       ([200], [1900])])
+def test_prompt_of_few_queries_over_many_keys(dev, dt, heads, kv, D, lens, past, causal):
+    """The keys split among blocks and joined; sequences shorter than the splits among them."""
+    q, k, v, cu, cu_k = _prompt_case(lens, heads, kv, D, dt, 12, past)
+    from helix_substrate import _hxq
+    assert _hxq._prompt_workspace(sum(lens), k.shape[0], len(lens), heads, D, 0) > 0
+    out = torch.full((sum(lens) + 4, heads, D), 3.0, dtype=dt, device=dev)
+    pad = torch.cat([q, torch.full((4, heads, D), math.nan, dtype=dt)])
+    got = attn_prompt(pad.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu_k.to(dev), causal=causal, out=out)
+    assert (got[sum(lens):] == 3).all()
+    _check_prompt(got[:sum(lens)], q, k, v, cu, cu_k, causal=causal)
+    bad = v.clone()
+    bad[int(cu_k[1]) - 1, 0, 7] = math.nan       # the first sequence's last key: its last query only
+    got2 = attn_prompt(pad.to(dev), k.to(dev), bad.to(dev), cu.to(dev), cu_k.to(dev), causal=causal, out=out.clone())
+    group, last = heads // kv, lens[0] - 1
+    if causal:
+        assert torch.equal(got2[:last], got[:last])
+    assert got2[last, :group, 7].isnan().all()
+    assert torch.equal(got2[lens[0]:], got[lens[0]:])
+
+
 def test_prompt_long(dev):
     q, k, v, cu, _ = _prompt_case([2500, 700], 4, 1, 128, BF, 3)
     got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), scale=0.11)
