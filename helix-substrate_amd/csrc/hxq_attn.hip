@@ -384,7 +384,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
     using B0 = std::integral_constant<int, 0>;
     using B1 = std::integral_constant<int, NB - 1>;
     int t = t0;
-    for (; t < min(clean, t1); t += NB) {
+    for (; t < (SPLIT ? min(clean, t1) : clean); t += NB) {   // (with the min 3 % slower where it is not needed)
         step(t, B0{}, std::false_type{});
         if constexpr (NB == 2) step(t + 1, B1{}, std::false_type{});
     }
