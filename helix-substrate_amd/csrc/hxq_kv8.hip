@@ -131,6 +131,8 @@ struct AppendArgs {
 
 constexpr int kQHeads = 4;   // query heads a block of rows is rotated for at once
 
+// HBM bound in large calls: 28 + 8 heads, 48 ragged pieces in fp32 (581 MB) 123 us, 4.7 TB/s; a prompt of 1000
+// rows (11 MB) 9.8 us, a chain of offsets, rows, rotation, maximum, store.
 // One block per (64 cache slots of a sequence, kv head or kQHeads query heads).  A thread owns 8
 // neighbouring pairs (i, i + D/2) of a row, so that every access is 16 bytes.
 // The block that completes the unfinished one reads the tail; the sequence's last, again unfinished
@@ -344,6 +346,9 @@ __device__ __forceinline__ float rows_sum(float v) {
 }
 
 // One block: 8 waves over the units of a split of one (sequence, kv head, tile of 8 query heads).
+// HBM bound: 64 sequences of 800 to 16000 tokens, 28 heads over 4 (564 MB) 124 us, 4.55 TB/s; one of 131000,
+// 16 over 2 (67 MB) 15.8 us, of which 3 to 5 are the start (arguments, counts, token, rotation); one of 500
+// 9.7 us.
 //
 // A wave takes a unit of 64 tokens by itself, in registers, with v_mfma_f32_16x16x32_bf16:
 //   S^T = K q^T: rows are tokens, columns are heads.  Row 4 k + r of tile j is given the token
@@ -810,7 +815,8 @@ __device__ __forceinline__ uint32_t weight_key(float v) {
 }
 
 // One block per (sequence, kv head): the least weight that stays by four passes over its bits
-// (histograms of 8 bits), then one pass in order that gives every block its new place.
+// (histograms of 8 bits), then one pass in order that gives every block its new place.  Latency bound: 256
+// rows of 2047 blocks 8.5 us, 2 of 157 4.4 us.
 __global__ __launch_bounds__(kEvThr) void kv8_evict_kernel(const float *weight, const int32_t *blocks,
                                                            const int32_t *cached, int32_t n_kv, int32_t n_blocks,
                                                            int32_t keep, int32_t sink, int32_t recent, float *w_out,

@@ -864,7 +864,8 @@ def attn_prompt(q, k, v, cu_q, cu_k, scale, causal, out):
                            f"{out.dtype})")
     if ks != v.shape or ks[2] != qs[2] or out.shape != qs:
         raise ValueError("shapes must be q, out [rows, heads, D], k, v [rows, kv heads, D]")
-    _need_i32(cu_q=cu_q, cu_k=cu_k)
+    if cu_q.dtype != torch.int32 or (cu_k is not None and cu_k.dtype != torch.int32):
+        raise RuntimeError("cu_q and cu_k must be int32")
     if cu_q.dim() != 1 or cu_q.numel() < 1 or (cu_k is not None and cu_k.shape != cu_q.shape):
         raise ValueError("cu_q and cu_k must be [n_seqs + 1]")
     if cu_k is None and ks[0] != qs[0]:
@@ -872,10 +873,12 @@ def attn_prompt(q, k, v, cu_q, cu_k, scale, causal, out):
     n_seqs, rows, rows_k, heads, D = cu_q.numel() - 1, qs[0], ks[0], qs[1], qs[2]
     nbytes = _prompt_workspace(rows, rows_k, n_seqs, heads, D, dev)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
-    _call_on(dev, "hxq_attn_prompt", q.data_ptr(), *_steps(qs, qt), k.data_ptr(), *_steps(ks, kt),
-             v.data_ptr(), *_steps(ks, vt), dtype_code(dt), cu_q.data_ptr(), _ptr(cu_k), n_seqs,
-             rows, rows_k, heads, ks[1], D, scale, causal, out.data_ptr(), *_steps(qs, ot),
-             _ptr(ws), nbytes, _stream(q))
+    if rows <= 1 or rows_k <= 1 or heads == 1 or ks[1] == 1:   # strides that no element needs: 0
+        qt, kt, vt, ot = _steps(qs, qt), _steps(ks, kt), _steps(ks, vt), _steps(qs, ot)
+    _call_on(dev, "hxq_attn_prompt", q.data_ptr(), qt[0], qt[1], k.data_ptr(), kt[0], kt[1],
+             v.data_ptr(), vt[0], vt[1], dtype_code(dt), cu_q.data_ptr(), _ptr(cu_k), n_seqs, rows,
+             rows_k, heads, ks[1], D, scale, causal, out.data_ptr(), ot[0], ot[1], _ptr(ws), nbytes,
+             _stream(q))
     return out
 
 
@@ -936,18 +939,23 @@ def kv8_append(q, k, v, cu_rows, cached, pos, theta, desc, q_out, k_out, v_out):
         raise ValueError("q must be [rows, heads, D], k and v [rows, kv heads, D] of the cache")
     if dt != v.dtype or (q is not None and q.dtype != dt):
         raise RuntimeError("q, k and v must have one dtype")
-    _need_i32(cu_rows=cu_rows, cached=cached, pos=pos)
-    batch = desc.batch
+    batch, i32 = desc.batch, torch.int32
+    if not (cu_rows.dtype == cached.dtype == i32 and (pos is None or pos.dtype == i32)):
+        raise RuntimeError("cu_rows, cached and pos must be int32")
     if cu_rows.shape != (batch + 1,) or cached.shape != (batch,) or (
-            pos is not None and pos.shape != cached.shape):
+            pos is not None and pos.shape != (batch,)):
         raise ValueError("cu_rows must be [batch + 1], cached and pos [batch]")
-    for t, like in ((q_out, qs if q is not None else None), (k_out, ks), (v_out, ks)):
-        if t is not None and (t.shape != like or _DTYPE_CODE.get(t.dtype) != desc.dtype):
-            raise ValueError("outputs must have the rows' shapes and the cache's 16-bit dtype")
-    _call_on(dev, "hxq_kv8_append", _ptr(q), *_steps(qs, qt), k.data_ptr(), *_steps(ks, kt),
-             v.data_ptr(), *_steps(ks, vt), dtype_code(dt), cu_rows.data_ptr(), ks[0], qs[1],
-             cached.data_ptr(), _ptr(pos), theta, ctypes.addressof(desc), _ptr(q_out), _ptr(k_out),
-             _ptr(v_out), _stream(k))
+    c16 = desc.dtype
+    if not ((q_out is None or (q is not None and q_out.shape == qs and _KV16.get(q_out.dtype) == c16))
+            and (k_out is None or (k_out.shape == ks and _KV16.get(k_out.dtype) == c16))
+            and (v_out is None or (v_out.shape == ks and _KV16.get(v_out.dtype) == c16))):
+        raise ValueError("outputs must have the rows' shapes and the cache's 16-bit dtype")
+    if ks[0] == 1 or ks[1] == 1 or qs[1] == 1:   # strides that no element needs count as 0
+        qt, kt, vt = _steps(qs, qt), _steps(ks, kt), _steps(ks, vt)
+    _call_on(dev, "hxq_kv8_append", _ptr(q), qt[0], qt[1], k.data_ptr(), kt[0], kt[1], v.data_ptr(),
+             vt[0], vt[1], dtype_code(dt), cu_rows.data_ptr(), ks[0], qs[1], cached.data_ptr(),
+             _ptr(pos), theta, ctypes.addressof(desc), _ptr(q_out), _ptr(k_out), _ptr(v_out),
+             _stream(k))
 
 
 def kv8_attn_decode(q, k, v, cached, pos, theta, scale, desc, weight, weight_out, out):

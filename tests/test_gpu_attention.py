@@ -611,3 +611,119 @@ def test_on_another_stream(dev):
         got = attn_prompt(*a)
     s.synchronize()
     assert torch.equal(got, want)
+
+
+def test_attend_and_append_offsets_past_32_bits(dev):
+    """A cache of 4.9 GB of keys: the first blocks of the order lie at its end."""
+    kv, D, n, heads, past = 1, 128, 600_000, 4, 200
+    big = HelixKV8Cache.empty(1, kv, D, n * BLOCK, device=dev)
+    big.blocks.copy_(big.blocks.flip(-1))
+    small = HelixKV8Cache.empty(1, kv, D, 5 * BLOCK, device=dev)
+    x = _rows(past, heads, kv, D, BF, 71).to(dev)
+    t = _rows(1, heads, kv, D, F32, 72).to(dev)
+    cut = lambda x: (x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:])
+    outs = []
+    for c in (big, small):
+        c.append(*cut(x), _i32([0], dev), _i32([0, past], dev), theta=1e6)
+        outs.append(c.attend(*cut(t), _i32([past], dev), theta=1e6)[0])
+    assert torch.equal(*outs)
+    assert big.k.numel() > 1 << 32
+    assert torch.equal(big.k[0, 0, n - 3:].flip(0).view(torch.uint8), small.k[0, 0, :3].view(torch.uint8))
+
+
+def test_two_calls_at_once(dev):
+    """Two streams: prompts and tokens of different caches, each as alone."""
+    heads, kv, D, past = 16, 2, 128, 3000
+    cut = lambda x: (x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:])
+    caches = [_filled(1, kv, D, BF, [past], 50, dev, 80 + i) for i in range(2)]
+    xs = [_rows(1, heads, kv, D, F32, 90 + i).to(dev) for i in range(2)]
+    prompts = [_prompt_case([9], heads, kv, D, BF, 95 + i, [4000]) for i in range(2)]
+    prompts = [[t.to(dev) for t in p] for p in prompts]
+    run = lambda i: (caches[i].attend(*cut(xs[i]), _i32([past], dev), theta=1e6,
+                                      weight_out=caches[i].new_weight()), attn_prompt(*prompts[i]))
+    want = [run(i) for i in range(2)]
+    streams = [torch.cuda.Stream(device=dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(run(i))
+        torch.cuda.synchronize()
+        for (a, p), (b, r) in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(p, r)
+
+
+def test_prompt_captured_and_replayed(dev):
+    """The form with split keys, its workspace from the graph's pool."""
+    q, k, v, cu, cu_k = (t.to(dev) for t in _prompt_case([5, 40], 16, 2, 128, BF, 99, [3000, 2000]))
+    want = attn_prompt(q, k, v, cu, cu_k)
+    s, g = torch.cuda.Stream(device=dev), torch.cuda.CUDAGraph()
+    s.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+        out = attn_prompt(q, k, v, cu, cu_k)
+    torch.cuda.current_stream(dev).wait_stream(s)
+    for i in range(4):
+        out.zero_()
+        g.replay()
+        torch.randn(1 << 20, device=dev).sum().item()
+        assert torch.equal(out, want)
+
+
+def test_prompt_over_its_queries(dev):
+    """out may be q."""
+    q, k, v, cu, _ = _prompt_case([300, 77], 8, 2, 128, BF, 101)
+    a = [t.to(dev) for t in (q, k, v, cu)]
+    want = attn_prompt(*a)
+    assert torch.equal(attn_prompt(*a, out=a[0]), want) and torch.equal(a[0], want)
+
+
+def test_refusals_of_the_wrappers(dev):
+    q, k, v, cu, _ = (t.to(dev) for t in _prompt_case([20], 4, 2, 64, BF, 102))
+    with pytest.raises(RuntimeError, match="one dtype"):
+        attn_prompt(q, k.half(), v, cu)
+    with pytest.raises(RuntimeError, match="one dtype"):
+        attn_prompt(q, k, v, cu, out=torch.empty_like(q, dtype=F32))
+    with pytest.raises(ValueError, match="shapes"):
+        attn_prompt(q, k, v[:, :1], cu)
+    with pytest.raises(RuntimeError, match="int32"):
+        attn_prompt(q, k, v, cu.long())
+    with pytest.raises(RuntimeError, match="device tensors"):
+        attn_prompt(q, k, v, cu.cpu())
+    with pytest.raises(ValueError, match="cu_q and cu_k"):
+        attn_prompt(q, k, v, cu, cu[:1])
+    with pytest.raises(ValueError, match="as many rows"):
+        attn_prompt(q, k[:10], v[:10], cu)
+    with pytest.raises(RuntimeError, match="multiples of 16"):
+        attn_prompt(q, k.view(-1)[4:4 + 19 * 128].view(19, 2, 64), v[:19], cu, cu)
+    with pytest.raises(RuntimeError, match="head_dim"):
+        attn_prompt(*(t[..., :32].contiguous() for t in (q, k, v)), cu)
+    cache = HelixKV8Cache.empty(2, 2, 64, 128, device=dev)
+    n = _i32([0, 0], dev)
+    with pytest.raises(ValueError, match="of the cache"):
+        cache.attend(q[:3], k[:3], v[:3], n)
+    with pytest.raises(RuntimeError, match="int32"):
+        cache.attend(q[:2], k[:2], v[:2], n.long())
+    with pytest.raises(RuntimeError, match="int32"):
+        cache.attend(q[:2], k[:2], v[:2], n[:1])
+    with pytest.raises(ValueError, match="fp32"):
+        cache.attend(q[:2], k[:2], v[:2], n, weight_out=torch.zeros(2, 2, 3, device=dev))
+    with pytest.raises(RuntimeError, match="weight_in"):
+        cache.attend(q[:2], k[:2], v[:2], n, weight=cache.new_weight())
+    with pytest.raises(ValueError, match="cu_rows"):
+        cache.append(q, k, v, n, cu)
+    with pytest.raises(ValueError, match="16-bit dtype"):
+        cache.append(q, k, v, n, _i32([0, 5, 20], dev), outs=(q.float(), None, None))
+    with pytest.raises(RuntimeError, match="one dtype"):
+        cache.append(q.float(), k, v, n, _i32([0, 5, 20], dev))
+    with pytest.raises(RuntimeError, match="must hold|keep"):
+        kv8_evict(cache.new_weight(), cache.blocks, n, 1, sink=1, recent=1)
+    with pytest.raises(RuntimeError, match="e4m3"):
+        HelixKV8Cache(cache.k.view(torch.uint8), cache.v, cache.k_scale, cache.v_scale, cache.k_tail,
+                      cache.v_tail)
+    with pytest.raises(ValueError, match="fit together"):
+        HelixKV8Cache(cache.k, cache.v, cache.k_scale[:1], cache.v_scale, cache.k_tail, cache.v_tail)
+    with pytest.raises(ValueError, match="block table"):
+        HelixKV8Cache.empty(1, 1, 64, 64, device=dev, table=False).evict(cache.new_weight(), n, 1)
+    with pytest.raises(ValueError, match="within the cache"):
+        cache.read(0, 129)
