@@ -66,9 +66,9 @@ def test_prompt(dev, dt, heads, kv, D, lens):
 
 
 def _behind(q, n_seqs):
-    """q with rows of no sequence behind it, to 1536 rows a sequence: a large call, which the 8-wave
+    """q with rows of no sequence behind it, to 1600 rows a sequence: a large call, which the 8-wave
     blocks take (from 64 heads on)."""
-    more = torch.full((max(1536 * n_seqs - q.shape[0], 0), *q.shape[1:]), math.nan, dtype=q.dtype)
+    more = torch.full((max(1600 * n_seqs - q.shape[0], 0), *q.shape[1:]), math.nan, dtype=q.dtype)
     return torch.cat([q, more])
 
 
