@@ -14,6 +14,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
+constexpr int64_t kMaxThreads = int64_t{1} << 32;   // a launch has fewer in x
+
 // [rows, heads, head_dim] with strides in elements
 struct HeadRows {
     const void *p;

@@ -160,9 +160,13 @@ __device__ __forceinline__ void add_odd(const uint16_t *row, bool seen, f32x16 (
         }
 }
 
+// What the weights are divided by: no key seen gives zeros; keys seen but every score -inf, NaN as 0 / 0.
+__device__ __forceinline__ float inv_sum(float sum, bool sees) {
+    return sum > 0.f || sum != sum ? 1.f / sum : sees ? __uint_as_float(0x7fc00000u) : 0.f;
+}
+
 template <bool BF16, int ND>
-__device__ __forceinline__ void store_rows(const f32x16 (&o)[ND], float sum, uint16_t *to) {
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;   // no key seen: zeros
+__device__ __forceinline__ void store_rows(const f32x16 (&o)[ND], float inv, uint16_t *to) {
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
@@ -419,7 +423,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
                 *reinterpret_cast<f32x4 *>(to + 32 * i + 2 * r) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
         if (hh == 0) a.ml[at] = float2{m * a.scale2, l};
     } else {
-        store_rows<BF16, ND>(o, l, static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)(q_beg + iq) * a.out_row + 4 * hh);
+        store_rows<BF16, ND>(o, inv_sum(l, lim >= 0), static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)(q_beg + iq) * a.out_row + 4 * hh);
     }
 }
 
@@ -452,7 +456,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const PromptArgs a) {
     // a split of which the query sees nothing has sum 0 (and NaN where all that it sees is NaN)
     const float f = e.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(e.x - mm);
     const float ll = wave_sum(f * e.y);
-    const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
+    const float inv = inv_sum(ll, keys_seen<CAUSAL>(i, at.lq, at.lk) > 0);
     uint16_t *to = static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)(at.q_beg + i) * a.out_row + lane * R;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -517,7 +521,7 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
     HXQ_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads");
     HXQ_REQUIRE(n_seqs >= 0 && rows_q >= 0 && rows_k >= 0 && rows_q < (int64_t{1} << 31) - 1024 &&
                     rows_k < (int64_t{1} << 31) - 1024, "bad sizes");
-    HXQ_REQUIRE(scale == scale && scale > 0.f && scale < INFINITY, "scale must be positive and finite");
+    HXQ_REQUIRE(scale >= 0x1p-100f && scale <= 0x1p100f, "scale must lie in 2^-100 .. 2^100");
     if (n_seqs == 0 || rows_q == 0) return HXQ_OK;
     HXQ_REQUIRE(q && out && cu_q && (rows_k == 0 || (k && v)), "q, k, v, cu_q and out are required");
     const HeadRows qr{q, q_row_stride, q_head_stride}, kr{k, k_row_stride, k_head_stride}, vr{v, v_row_stride, v_head_stride},
@@ -534,12 +538,13 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
     // us by die, 23 round)
     const bool by_die = tiles * n_kv_heads >= 64;
     const int64_t blocks = by_die ? (tiles * n_kv_heads + 7) / 8 * 8 * (n_heads / n_kv_heads) : tiles * n_heads;
-    HXQ_REQUIRE(blocks < (int64_t{1} << 31), "too many rows");
+    const int64_t joins = plan.splits > 1 ? tiles * n_heads * 32 : 0;
+    HXQ_REQUIRE(blocks * 64 * plan.nw < kMaxThreads && joins * 256 < kMaxThreads, "too many rows, sequences or heads");
     const PromptArgs a{qr, kr, vr, out, out_row_stride, out_head_stride, cu_q, cu_k ? cu_k : cu_q, n_seqs,
                        static_cast<int32_t>(rows_q), static_cast<int32_t>(rows_k), n_heads, n_heads / n_kv_heads,
                        scale * 1.44269504088896340736f, plan.splits, by_die, static_cast<float *>(workspace),
                        reinterpret_cast<float2 *>(static_cast<char *>(workspace) + plan.part_bytes)};
-    const dim3 grid(static_cast<uint32_t>(blocks), plan.splits), join(static_cast<uint32_t>(plan.splits > 1 ? tiles * n_heads * 32 : 0));
+    const dim3 grid(static_cast<uint32_t>(blocks), plan.splits), join(static_cast<uint32_t>(joins));
     const auto go = [&](auto bf, auto dd) {
         constexpr bool B = decltype(bf)::value;
         constexpr int D = decltype(dd)::value;

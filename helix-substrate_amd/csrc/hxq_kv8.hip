@@ -701,8 +701,8 @@ constexpr int kFewSplits = 16;   // up to here a wave joins a query head by itse
 
 // What is left when the splits are done.  The first `row_blocks` blocks join the splits of query heads:
 // a wave each, with no exchange (64 sequences, 28 heads, 4 splits: 5.4 us against 8.7 with a block
-// each), or a block each where there are many splits.  The others: weight_out = weight_in + every cache block's share of the softmax, kThr cache
-// blocks of one (sequence, kv head) each.
+// each), or a block each where there are many splits.  The others: weight_out = weight_in + every
+// cache block's share of the softmax, kThr cache blocks of one (sequence, kv head) each.
 template <int D>
 __global__ __launch_bounds__(kThr) void kv8_join_kernel(const DecodeArgs a, const int row_blocks) {
     constexpr int Q = D / 4, NG = kThr / Q, NW = kThr / kWave;
@@ -986,7 +986,7 @@ extern "C" int hxq_kv8_append(const void *q, int64_t q_row_stride, int64_t q_hea
     const AppendArgs a{qr, kr, vr, cu_rows, cached, pos, rope_table(theta, cache->head_dim), static_cast<int32_t>(rows), n_heads, *cache, q_out, k_out, v_out};
     const int64_t tiles = rows / kBlk + 2 * (int64_t)cache->batch;
     const int64_t heads = cache->n_kv_heads + (q_out ? (n_heads + kQHeads - 1) / kQHeads : 0);
-    HXQ_REQUIRE(tiles < (int64_t{1} << 31) && heads <= 65535, "too many rows or heads");
+    HXQ_REQUIRE(tiles * kThr < kMaxThreads && heads <= 65535, "too many rows, sequences or heads");
     const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(heads));
     kv8_dispatch(dtype, *cache, [&](auto dt, auto bf, auto d) {
         hipLaunchKernelGGL((kv8_append_kernel<decltype(dt)::value, decltype(bf)::value, decltype(d)::value>), grid,
@@ -998,7 +998,8 @@ extern "C" int hxq_kv8_append(const void *q, int64_t q_row_stride, int64_t q_hea
 
 extern "C" int64_t hxq_kv8_attn_decode_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
                                                        int32_t head_dim, int32_t n_blocks, int32_t weights) {
-    if (batch <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_blocks <= 0) return -1;
+    if (batch <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_blocks <= 0 ||
+        (head_dim != 64 && head_dim != 128)) return -1;
     const int s = kv8_splits(kv8_tiles(batch, n_heads, n_kv_heads), n_blocks);
     return kv8_ws(batch, n_heads, s, head_dim, n_blocks, weights != 0).bytes;
 }
@@ -1014,7 +1015,8 @@ extern "C" int hxq_kv8_attn_decode(const void *q, int64_t q_row_stride, int64_t 
     HXQ_REQUIRE(q && k && v && cached && out, "q, k, v, cached and out are required");
     HXQ_REQUIRE(attn_dtype(dtype, true) && attn_dtype(out_dtype, true), "bad dtype");
     HXQ_REQUIRE(n_heads > 0 && n_heads % cache->n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads");
-    HXQ_REQUIRE(theta >= 0.f && theta < INFINITY && scale == scale && fabsf(scale) < INFINITY, "theta and scale must be finite");
+    HXQ_REQUIRE(theta >= 0.f && theta < INFINITY && fabsf(scale) <= 0x1p100f,
+                "theta must be finite and not negative, scale finite and at most 2^100");
     HXQ_REQUIRE(weight_out || !weight_in, "weight_in without weight_out");
     const int64_t tiles = kv8_tiles(cache->batch, n_heads, cache->n_kv_heads);
     HXQ_REQUIRE(cache->batch <= 65535 && tiles / cache->batch <= 65535 && (int64_t)cache->batch * n_heads < (int64_t{1} << 31), "batch or heads too large");
@@ -1031,7 +1033,7 @@ extern "C" int hxq_kv8_attn_decode(const void *q, int64_t q_row_stride, int64_t 
     // what the second launch has to do: rows to join, chunks of weights
     const int64_t rows = (int64_t)cache->batch * n_heads;
     const int64_t chunks = weight_out ? (int64_t)cache->batch * cache->n_kv_heads * ((cache->n_blocks + kThr - 1) / kThr) : 0;
-    HXQ_REQUIRE(rows + chunks < (int64_t{1} << 31), "batch * heads or blocks too large");
+    HXQ_REQUIRE((rows + chunks) * kThr < kMaxThreads, "batch * heads or blocks too large");
     const int64_t row_blocks = splits == 1 ? 0 : splits <= kFewSplits ? (rows + kThr / kWave - 1) / (kThr / kWave) : rows;
     const dim3 join(static_cast<uint32_t>(row_blocks + chunks));
     const dim3 grid(splits, static_cast<uint32_t>(tiles / cache->batch), cache->batch);
@@ -1054,7 +1056,7 @@ extern "C" int hxq_kv8_evict(const float *weight, const int32_t *blocks_in, cons
     HXQ_REQUIRE(weight && cached && weight_out && blocks_out && cached_out, "weight, cached and the outputs are required");
     HXQ_REQUIRE(weight != weight_out && blocks_in != blocks_out && cached != cached_out, "outputs must not be the inputs");
     HXQ_REQUIRE(batch > 0 && n_kv_heads > 0 && n_blocks > 0 && n_blocks <= (1 << 24) &&
-                    (int64_t)batch * n_kv_heads < (int64_t{1} << 31), "bad sizes");
+                    (int64_t)batch * n_kv_heads * kEvThr < kMaxThreads, "bad sizes");
     HXQ_REQUIRE(keep > 0 && sink >= 0 && recent >= 0 && (int64_t)sink + recent <= keep,
                 "keep must be positive and hold the first `sink` and the last `recent` blocks");
     hipLaunchKernelGGL(kv8_evict_kernel, dim3(batch * n_kv_heads), dim3(kEvThr), 0, stream, weight, blocks_in, cached,

@@ -39,7 +39,8 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None):
 def rope_rows(q, k, v, cu_rows, pos, theta, dtype=torch.bfloat16, outs=None):
     """Rows of packed prompts rotated to positions pos[s], pos[s] + 1, ... (q and k; v is only
     rounded), in a 16-bit dtype: what ``HelixKV8Cache.append`` does, without a cache.  outs: three
-    tensors (or None) to write to, rows of a 16-bit cache for instance.  Returns (q, k, v)."""
+    tensors (or None) to write to, rows of a 16-bit cache for instance.  Returns (q, k, v); rows of
+    no sequence, or of one with a negative pos, are not written."""
     if outs is None:
         outs = tuple(None if t is None else torch.empty(t.shape, dtype=dtype, device=t.device)
                      for t in (q, k, v))
@@ -125,7 +126,8 @@ class HelixKV8Cache:
         """Rows of packed prompts behind the cached tokens: q and k are rotated to positions pos,
         pos + 1, ... (None: cached; theta 0: not rotated), k and v stored.  Returns the rows in the
         cache's 16-bit dtype (q, k, v), which `attn_prompt` takes; q None gives None.  outs: three
-        tensors (or None) to write them to.  Tokens past max_tokens are not stored."""
+        tensors (or None) to write them to; rows of no sequence, or of one with a negative cached,
+        are not written.  Tokens past max_tokens are not stored."""
         if outs is None:
             dt = self.dtype
             outs = (None if q is None else q.new_empty(q.shape, dtype=dt),
@@ -138,7 +140,8 @@ class HelixKV8Cache:
         """One token of each sequence: rotate q and k to pos (None: cached), store k and v behind
         the cached tokens, and attend over them and the token itself.  weight_out gets weight
         (None: zeros) plus each block's share of the softmax summed over the query heads of its kv
-        head; it may be weight.  Returns (out [batch, heads, D], weight_out)."""
+        head; it may be weight.  Returns (out [batch, heads, D], weight_out); a sequence with a
+        negative cached is skipped, its part of both not written.  One with no room left gives NaN."""
         if out is None:
             out = q.new_empty(q.shape, dtype=out_dtype)
         _hxq.kv8_attn_decode(q, k, v, cached, pos, theta,

@@ -540,12 +540,13 @@ int hxq_argmax(const float *logits, int64_t n, int32_t *out_id, int32_t *pos,
  *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j]) v[j]
  * over the sequence's keys j; causal: j <= i + (keys - queries), both counted in the sequence, so a
  * prompt that continues cached tokens passes them as its first keys.  A query that sees no key
- * gives zeros.  Keys that a query does not see have no influence, whatever they hold.  dtype (q, k,
- * v, out): HXQ_BF16 or HXQ_F16; scores, softmax and sums are fp32, the softmax weights are rounded
- * to dtype before the product with v.  Rows of out that belong to no sequence are left as they
- * were; offsets are clamped to [0, rows_q] and [0, rows_k].  scale > 0.  Row strides of k and v: 0 to
- * 2^24 - 1 elements.  out may be q, and must not overlap k or v.  workspace: device scratch of hxq_attn_prompt_workspace_bytes(...) bytes (0 but for few
- * queries over many keys), written and read within the call.
+ * gives zeros; one whose scores are all -inf gives NaN.  Keys that a query does not see have no
+ * influence, whatever they hold.  dtype (q, k, v, out): HXQ_BF16 or HXQ_F16; scores, softmax and sums
+ * are fp32, the softmax weights are rounded to dtype before the product with v.  Rows of out that
+ * belong to no sequence are left as they were; offsets are clamped to [0, rows_q] and [0, rows_k].
+ * scale: 2^-100 to 2^100.  Row strides of k and v: 0 to 2^24 - 1 elements.  out may be q, and must
+ * not overlap k or v.  workspace: device scratch of hxq_attn_prompt_workspace_bytes(...) bytes (0 but
+ * for few queries over many keys), written and read within the call.
  */
 int64_t hxq_attn_prompt_workspace_bytes(int64_t rows_q, int64_t rows_k, int32_t n_seqs,
                                         int32_t n_heads, int32_t head_dim);
@@ -611,13 +612,16 @@ int hxq_kv8_append(const void *q, int64_t q_row_stride, int64_t q_head_stride, c
  * One token of each sequence: rotation (as hxq_kv8_append), its key and value into the cache, and
  * its attention over the cached tokens and itself, out [batch, n_heads, D] (contiguous, any
  * hxq_dtype).  Full blocks are read in 8 bits, the unfinished block and the token in 16 bits; the
- * token that ends a block still sees it in 16 bits.  q keeps its fp32 bits after the rotation.
+ * token that ends a block still sees it in 16 bits.  q keeps its fp32 bits after the rotation.  Keys
+ * and values that are not finite count as NaN (infinities of the unfinished block as NaN or as
+ * themselves): out is NaN in the heads that read such a key, in a value's dimension.
  * weight_out (optional) fp32 [batch, n_kv_heads, n_blocks]: weight_in plus each block's share of
  * the softmax, summed over the query heads of the kv head (entry j: the j-th block in order, the
  * unfinished one included); weight_in NULL = zeros, weight_out may be weight_in.  A sequence with
  * cached >= n_blocks * 64 has no room: its out is NaN, its cache and weights stay.  A block table
- * entry outside [0, n_blocks) makes the sequence's out NaN.  workspace: device scratch of
- * hxq_kv8_attn_decode_workspace_bytes(...) bytes, written and read within the call.
+ * entry outside [0, n_blocks) makes out and weights NaN for the heads that read it.  |scale| is at
+ * most 2^100.  workspace: device scratch of hxq_kv8_attn_decode_workspace_bytes(...) bytes, written
+ * and read within the call.
  */
 int64_t hxq_kv8_attn_decode_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
                                             int32_t head_dim, int32_t n_blocks, int32_t weights);

@@ -44,6 +44,23 @@ def test_prompt_refuses(lib, change, text):
     assert text in _message(lib)
 
 
+@pytest.mark.parametrize("change,text", [
+    (dict(scale=2.0 ** -101), "scale"), (dict(scale=2.0 ** 101), "scale"),
+    (dict(n=1 << 21), "too many"),                                # 2^21 sequences, 16 heads, 256 threads
+    (dict(heads=2, kv=2, rows_k=(1 << 30), n=1 << 19, ws=A, ws_bytes=1 << 40), "too many")])   # the join
+def test_prompt_refuses_what_a_launch_cannot_hold(lib, change, text):
+    assert lib.hxq_attn_prompt(*{**PROMPT, **change}.values()) == 1
+    assert text in _message(lib)
+
+
+def test_cache_launches_too_large(lib):
+    assert _append(lib, _desc(batch=1 << 24)) == 1 and "too many" in _message(lib)
+    assert _attend(lib, _desc(batch=65535, n_blocks=1 << 24), ws_bytes=1 << 60) == 1 and "too large" in _message(lib)
+    assert lib.hxq_kv8_evict(*{**EVICT, "batch": 1 << 21}.values()) == 1 and "sizes" in _message(lib)
+    assert _attend(lib, _desc(), scale=2.0 ** 101) == 1 and "scale" in _message(lib)
+    assert lib.hxq_kv8_attn_decode_workspace_bytes(1, 16, 2, 96, 4, 0) == -1
+
+
 def test_prompt_of_nothing(lib):
     assert lib.hxq_attn_prompt(*{**PROMPT, "n": 0}.values()) == 0
     assert lib.hxq_attn_prompt(*{**PROMPT, "rows_q": 0, "q": None}.values()) == 0

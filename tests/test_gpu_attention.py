@@ -171,6 +171,34 @@ def test_prompt_unseen_values_have_no_influence(dev, bad, lens, heads):
     _check_prompt(got, q, k, v, cu, cu)
 
 
+@pytest.mark.parametrize("lens,past,heads,bad", [
+    ([70, 200], [0, 0], 4, [0, 1, 5, 64, 70, 71, 130]),          # rows that see only -inf at the start
+    ([3], [2500], 4, list(range(1500))),                         # whole splits of -inf
+    ([3, 2], [2500, 0], 4, list(range(2503)))])                  # a sequence of nothing else
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_prompt_scores_of_minus_infinity(dev, dt, lens, past, heads, bad):
+    """A key whose score is -inf has weight 0; where every score is -inf, the softmax is 0 / 0."""
+    q, k, v, cu, cu_k = _prompt_case(lens, heads, 2, 64, dt, 23, past)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    k[bad, :, 3] = -math.inf
+    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu_k.to(dev)).cpu().double()
+    usable = torch.ones(len(k), dtype=torch.bool)
+    usable[bad] = False
+    h = ref.half_step(dt)
+    for s in range(len(lens)):
+        rq, rk = slice(int(cu[s]), int(cu[s + 1])), slice(int(cu_k[s]), int(cu_k[s + 1]))
+        seen = ref.causal(lens[s], lens[s] + past[s])
+        fine = seen & usable[rk]
+        kk, vv = k[rk].double().nan_to_num(neginf=0.0), v[rk].double()
+        out, _, spread, err = ref.attention(q[rq].double(), kk, vv, 64 ** -0.5, fine)
+        tol = h * out.abs() + (h + 2 * err + len(kk) * 2.0 ** -24) * spread * (1 + h) + 1e-30
+        if dt == FP:   # as above: subnormal weights
+            tol = tol + 2.0 ** -25 * vv.abs().sum(0).repeat_interleave(heads // 2, 0) + 2.0 ** -25
+        none = ~fine.any(1)
+        assert got[rq][none].isnan().all()
+        assert ((got[rq] - out).abs() <= tol)[~none].all()
+
+
 def test_prompt_neighbours_and_rows_behind(dev):
     """NaN in rows of no sequence reach nobody; their rows of out stay as they were."""
     q, k, v, cu, _ = _prompt_case([70, 60], 4, 2, 64, BF, 7)
