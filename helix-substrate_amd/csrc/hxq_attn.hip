@@ -192,7 +192,7 @@ __device__ __forceinline__ void store_rows(const f32x16 (&o)[ND], float inv, uin
 // is 14 %, the global loads 13 %, the LDS reads 10 %; the matrix pipe is busy half the time).  P in the
 // operands' 16 bits: half a step of each weight, of the size of the output's own rounding.  Measured:
 // 16 heads over 2, 16384 tokens 990 us (1.11 PFLOP/s); 28 over 4, twelve sequences of 371 to 2048 235;
-// fp16 at head_dim 64, six pieces over 7000 keys 112; 211 tokens 13.
+// fp16 at head_dim 64, six pieces over 7000 keys 106; 211 tokens 13.
 template <int NW, bool BF16, int D, bool CAUSAL, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArgs a) {
     constexpr int THR = 64 * NW, BM = 32 * NW, NB = NW == 8 ? 2 : 1;
@@ -243,7 +243,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
         const int per = steps_per_split(steps, a.splits);
         t0 = min(static_cast<int>(blockIdx.y) * per, steps);
         t1 = min(t0 + per, steps);
-        if (t0 == t1 && t0 > 0) return;   // no part; the first is written also where nothing is seen
+        if (t0 == t1 && t0 > 0) {   // nothing to do; the first split is written also where nothing is seen
+            if (iq < lq && hh == 0) a.ml[((int64_t)(q_beg + iq) * a.n_heads + head) * a.splits + blockIdx.y] = float2{-INFINITY, 0.f};
+            return;
+        }
     }
     if (threadIdx.x < 2 * ODD) odd[threadIdx.x >> 1][threadIdx.x & 1] = 0u;
 
@@ -421,51 +424,53 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
 #pragma unroll
             for (int r = 0; r < 16; r += 4)
                 *reinterpret_cast<f32x4 *>(to + 32 * i + 2 * r) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
-        if (hh == 0) a.ml[at] = float2{m * a.scale2, l};
+        if (hh == 0) a.ml[at] = float2{m * a.scale2, l == 0.f && lim >= 0 ? -0.f : l};   // -0: every score -inf
     } else {
         store_rows<BF16, ND>(o, inv_sum(l, lim >= 0), static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)(q_beg + iq) * a.out_row + 4 * hh);
     }
 }
 
-// The splits of every query joined: a wave for a query of a head (32 blocks for the 128 queries of a
-// tile of the kernel above).
-template <bool BF16, int D, bool CAUSAL>
+// The splits (at most NS) of every query of a head joined, D / 4 lanes each.  No search for its
+// sequence: a split that has no keys is marked by its sum 0, and rows between the first offset and the
+// last belong to some sequence.  All loads are asked for at once, for splits past the last those of the
+// last again (behind branches each waits for the one before: 8 queries in 15 splits 12 us, 3.9 so).
+template <bool BF16, int D, int NS>
 __global__ __launch_bounds__(256) void attn_join_kernel(const PromptArgs a) {
-    constexpr int R = D / kWave, BM = 128;
-    const int unit = blockIdx.x / 32, head = unit % a.n_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    PromptTile at;
-    if (!prompt_tile<BM>(a, unit / a.n_heads, at)) return;
-    const int last = min(at.tile * BM + BM, at.lq) - 1;
-    const int steps = (keys_seen<CAUSAL>(last, at.lq, at.lk) + kBN - 1) / kBN, per = steps_per_split(steps, a.splits);
-    const int n = max((steps + per - 1) / per, 1);
-    const int i = at.tile * BM + blockIdx.x % 32 * 4 + wave;
-    if (i > last) return;
-    const int64_t row = (int64_t)(at.q_beg + i) * a.n_heads + head;
-    const float2 e = lane < n ? a.ml[row * a.splits + lane] : float2{-INFINITY, 0.f};
-    const float *pt = a.part + row * a.splits * D + lane * R;
-    float p[kMaxSplits][R];
+    constexpr int G = D / 4;
+    const int lane = threadIdx.x % G, n = a.splits;
+    const int rows = a.rows_q * a.n_heads, row = min(static_cast<int>(blockIdx.x * (256 / G) + threadIdx.x / G), rows - 1);
+    const int64_t at = (int64_t)row * n;
+    float2 e = a.ml[at + min(lane, n - 1)];
+    f32x4 p[NS];
 #pragma unroll
-    for (int s = 0; s < kMaxSplits; ++s)
-        if (s < n)
-#pragma unroll
-            for (int r = 0; r < R; ++r) p[s][r] = pt[s * D + r];
+    for (int s = 0; s < NS; ++s) p[s] = *reinterpret_cast<const f32x4 *>(a.part + (at + min(s, n - 1)) * D + 4 * lane);
+    if (lane >= n) e = float2{-INFINITY, 0.f};
     float mm = e.x;
 #pragma unroll
-    for (int s = kMaxSplits / 2; s >= 1; s >>= 1) mm = fmaxf(mm, __shfl_xor(mm, s, kWave));
-    mm = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(mm)));
+    for (int s = NS / 2; s >= 1; s >>= 1) mm = fmaxf(mm, __shfl_xor(mm, s, NS));
+    mm = __shfl(mm, 0, G);
     // a split of which the query sees nothing has sum 0 (and NaN where all that it sees is NaN)
     const float f = e.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(e.x - mm);
-    const float ll = wave_sum(f * e.y);
-    const float inv = inv_sum(ll, keys_seen<CAUSAL>(i, at.lq, at.lk) > 0);
-    uint16_t *to = static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)(at.q_beg + i) * a.out_row + lane * R;
+    float ll = f * e.y;
+    int sees = e.y != 0.f || __float_as_int(e.y) < 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        float x = 0.f;
-#pragma unroll
-        for (int s = 0; s < kMaxSplits; ++s)
-            if (s < n) x = fmaf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s)), p[s][r], x);
-        to[r] = BF16 ? f32_to_bf16(x * inv) : f32_to_f16(x * inv);
+    for (int s = NS / 2; s >= 1; s >>= 1) {
+        ll += __shfl_xor(ll, s, NS);
+        sees |= __shfl_xor(sees, s, NS);
     }
+    const float inv = inv_sum(__shfl(ll, 0, G), __shfl(sees, 0, G));
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        const float fs = __shfl(f, s, G);
+        const bool has = __shfl(e.y, s, G) != 0.f;   // what is not written is not used
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = fmaf(fs, has ? p[s][r] : 0.f, x[r]);
+    }
+    const int i = row / a.n_heads, head = row % a.n_heads;
+    if (i < seq_off(a.cu_q, 0, a.rows_q) || i >= seq_off(a.cu_q, a.n_seqs, a.rows_q)) return;
+    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)i * a.out_row + 4 * lane) =
+        u32x2{pack16<BF16>(x[0] * inv, x[1] * inv), pack16<BF16>(x[2] * inv, x[3] * inv)};
 }
 
 }  // namespace hxq
@@ -481,19 +486,26 @@ struct PromptPlan {
 
 // What depends on sizes that the host knows; lengths of sequences are on the device.
 PromptPlan prompt_plan(int64_t rows_q, int64_t rows_k, int64_t n_seqs, int64_t n_heads, int32_t D) {
-    const int64_t cus = device_cu_count();
     PromptPlan p{4, 1, 0, 0};
     // 8 waves for long sequences whose blocks reach every compute unit, 4 for the others (16 heads over 2,
     // us with 4 and 8 waves: one of 4096 tokens 136 and 124, of 8192 335 and 305, eight of 2048 178 and 173;
     // sixteen of 1024 116 and 123, one of 211 13 and 17): two blocks of 4 a unit hide each other's start,
     // 8 waves stage half the bytes.
-    if (D == 128 && rows_q >= 1536 * n_seqs && rows_q / 256 * n_heads >= cus) p.nw = 8;
-    // Few queries over many keys: the keys are split until there are two blocks a compute unit, at least
-    // 512 keys each (16 heads, us with one block and split: 8 queries over 8000 keys 216 and 29, 512 over 8500
-    // 230 and 61, 1024 over 2048 62 and 43, a prompt of 1500 48 and 49).
-    const int64_t blocks = std::max(std::min(rows_q, n_seqs), (rows_q + 127) / 128) * n_heads;
-    if (p.nw == 4 && blocks < cus)
-        p.splits = static_cast<int>(std::max<int64_t>(1, std::min({2 * cus / blocks, rows_k / n_seqs / 512, int64_t{kMaxSplits}})));
+    if (D == 128 && rows_q >= 1536 * n_seqs && rows_q / 256 * n_heads >= device_cu_count()) p.nw = 8;
+    if (p.nw == 8) return p;
+    // Few blocks: the keys of each are split, to as many blocks as run at once (two a compute unit, at
+    // head_dim 64 three), while a split keeps 192 keys (at head_dim 64 256, and 640 past one block a unit:
+    // its steps are half the work).  16 heads, us with one block and split: 8 queries over 8000 keys 216
+    // and 24, 512 over 8500 230 and 60, 2048 over 2048 61 and 51, 1000 over 1000 34 and 30; at head_dim 64
+    // 2048 over 10000 137 and 115, 200 over 1200 22 and 18.
+    const int64_t cus = device_cu_count(), held = (D == 64 ? 3 : 2) * cus;
+    const int64_t seqs = std::min(rows_q, n_seqs);
+    const int64_t blocks = std::max(seqs, (rows_q + 64 * seqs) / 128) * n_heads;
+    const int64_t keys = rows_k / seqs - rows_q / seqs / 2;   // that a query sees
+    int64_t splits = std::max(std::min(cus / blocks, keys / 256), std::min(held / blocks, keys / (D == 64 ? 640 : 192)));
+    // (one sequence: its blocks are alike, three splits take two rounds for three: 2304 over 3304 98 and 83)
+    if (D == 128 && n_seqs == 1 && blocks > cus && blocks <= 2 * held / 3 && keys >= 3 * 512) splits = 3;
+    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)));
     if (p.splits > 1) {
         p.part_bytes = rows_q * n_heads * p.splits * D * 4;
         p.bytes = p.part_bytes + rows_q * n_heads * p.splits * 8;
@@ -538,7 +550,7 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
     // us by die, 23 round)
     const bool by_die = tiles * n_kv_heads >= 64;
     const int64_t blocks = by_die ? (tiles * n_kv_heads + 7) / 8 * 8 * (n_heads / n_kv_heads) : tiles * n_heads;
-    const int64_t joins = plan.splits > 1 ? tiles * n_heads * 32 : 0;
+    const int64_t joins = plan.splits > 1 ? (rows_q * n_heads * (head_dim / 4) + 255) / 256 : 0;
     HXQ_REQUIRE(blocks * 64 * plan.nw < kMaxThreads && joins * 256 < kMaxThreads, "too many rows, sequences or heads");
     const PromptArgs a{qr, kr, vr, out, out_row_stride, out_head_stride, cu_q, cu_k ? cu_k : cu_q, n_seqs,
                        static_cast<int32_t>(rows_q), static_cast<int32_t>(rows_k), n_heads, n_heads / n_kv_heads,
@@ -552,7 +564,13 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
             constexpr bool C = decltype(cc)::value;
             if (plan.splits > 1) {
                 hipLaunchKernelGGL((attn_prompt_kernel<4, B, D, C, true>), grid, dim3(256), 0, stream, a);
-                hipLaunchKernelGGL((attn_join_kernel<B, D, C>), join, dim3(256), 0, stream, a);
+                const auto joined = [&](auto ns) {
+                    hipLaunchKernelGGL((attn_join_kernel<B, D, decltype(ns)::value>), join, dim3(256), 0, stream, a);
+                };
+                if (plan.splits <= 2) joined(std::integral_constant<int, 2>{});
+                else if (plan.splits <= 4) joined(std::integral_constant<int, 4>{});
+                else if (plan.splits <= 8) joined(std::integral_constant<int, 8>{});
+                else joined(std::integral_constant<int, kMaxSplits>{});
                 return;
             }
             if constexpr (D == 128)

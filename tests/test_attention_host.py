@@ -47,7 +47,7 @@ def test_prompt_refuses(lib, change, text):
 @pytest.mark.parametrize("change,text", [
     (dict(scale=2.0 ** -101), "scale"), (dict(scale=2.0 ** 101), "scale"),
     (dict(n=1 << 21), "too many"),                                # 2^21 sequences, 16 heads, 256 threads
-    (dict(heads=2, kv=2, rows_k=(1 << 30), n=1 << 19, ws=A, ws_bytes=1 << 40), "too many")])   # the join
+    (dict(heads=64, kv=64, rows_k=(1 << 30), n=1 << 19, ws=A, ws_bytes=1 << 40), "too many")])
 def test_prompt_refuses_what_a_launch_cannot_hold(lib, change, text):
     assert lib.hxq_attn_prompt(*{**PROMPT, **change}.values()) == 1
     assert text in _message(lib)

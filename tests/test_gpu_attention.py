@@ -121,6 +121,29 @@ def test_prompt_of_few_queries_over_many_keys(dev, dt, heads, kv, D, lens, past,
     assert torch.equal(got2[lens[0]:], got[lens[0]:])
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dt,heads,kv,D,lens,past", [
+    (BF, 16, 2, 128, [2304], [1000]),                          # three splits, two rounds of blocks
+    (FP, 16, 4, 64, [300, 0, 512, 256], [2000, 1500, 900, 0]),   # two to three, of uneven tiles
+    (BF, 16, 2, 128, [1000], [0]), (BF, 16, 4, 64, [130, 7], [1000, 0])])
+def test_prompt_splits_of_larger_calls(dev, dt, heads, kv, D, lens, past, causal):
+    q, k, v, cu, cu_k = _prompt_case(lens, heads, kv, D, dt, 31, past)
+    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu_k.to(dev), causal=causal)
+    _check_prompt(got, q, k, v, cu, cu_k, causal=causal)
+
+
+@pytest.mark.parametrize("heads,kv,D", [(16, 2, 128), (4, 4, 64)])
+def test_prompt_splits_leave_other_rows(dev, heads, kv, D):
+    """Rows of no sequence before and behind, a sequence without keys and one without queries."""
+    q, k, v, _, _ = _prompt_case([40], heads, kv, D, BF, 37, [6000])
+    cu, cu_k = torch.tensor([5, 9, 9, 14, 33]), torch.tensor([100, 2500, 3000, 3000, 6040])
+    out = torch.full_like(q, 7.0).to(dev)
+    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.int().to(dev), cu_k.int().to(dev), out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert (got[:5] == 7).all() and (got[33:] == 7).all() and (got[9:14] == 0).all()
+    _check_prompt(got, q, k, v, cu, cu_k)
+
+
 def test_prompt_long(dev):
     q, k, v, cu, _ = _prompt_case([2500, 700], 4, 1, 128, BF, 3)
     got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), scale=0.11)
