@@ -30,8 +30,6 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None):
     continues cached tokens).  bf16 or fp16, head_dim 64 or 128; scale None = head_dim^-1/2.
     Returns out, [rows, heads, head_dim]; rows that belong to no sequence stay as they were in a
     given out, and are undefined in a new one."""
-    if out is None:
-        out = q.new_empty(q.shape)
     return _hxq.attn_prompt(q, k, v, cu_q, cu_k, q.shape[-1] ** -0.5 if scale is None else scale,
                             bool(causal), out)
 
@@ -41,23 +39,16 @@ def rope_rows(q, k, v, cu_rows, pos, theta, dtype=torch.bfloat16, outs=None):
     rounded), in a 16-bit dtype: what ``HelixKV8Cache.append`` does, without a cache.  outs: three
     tensors (or None) to write to, rows of a 16-bit cache for instance.  Returns (q, k, v); rows of
     no sequence, or of one with a negative pos, are not written."""
-    if outs is None:
-        outs = tuple(None if t is None else torch.empty(t.shape, dtype=dtype, device=t.device)
-                     for t in (q, k, v))
     desc = _hxq.HxqKv8(None, None, None, None, None, None, None, _hxq.dtype_code(dtype),
                        cu_rows.numel() - 1, k.shape[1], k.shape[2], 0)
-    _hxq.kv8_append(q, k, v, cu_rows, pos, None, theta, desc, *outs)
-    return outs
+    return _hxq.kv8_append(q, k, v, cu_rows, pos, None, theta, desc, outs)
 
 
 def kv8_evict(weight, blocks, cached, keep, sink=0, recent=0):
     """The blocks that stay when every sequence and kv head keeps at most `keep` full blocks: the
     first `sink`, the last `recent`, and the greatest weight between them.  Returns new (blocks,
     weight, cached) tensors; see ``HelixKV8Cache.evict`` for a cache that is cut in place."""
-    weight_out, cached_out = torch.empty_like(weight), torch.empty_like(cached)
-    blocks_out = torch.empty_like(weight, dtype=torch.int32)
-    _hxq.kv8_evict(weight, blocks, cached, keep, sink, recent, weight_out, blocks_out, cached_out)
-    return blocks_out, weight_out, cached_out
+    return _hxq.kv8_evict(weight, blocks, cached, keep, sink, recent)
 
 
 class HelixKV8Cache:
@@ -128,12 +119,7 @@ class HelixKV8Cache:
         cache's 16-bit dtype (q, k, v), which `attn_prompt` takes; q None gives None.  outs: three
         tensors (or None) to write them to; rows of no sequence, or of one with a negative cached,
         are not written.  Tokens past max_tokens are not stored."""
-        if outs is None:
-            dt = self.dtype
-            outs = (None if q is None else q.new_empty(q.shape, dtype=dt),
-                    k.new_empty(k.shape, dtype=dt), v.new_empty(v.shape, dtype=dt))
-        _hxq.kv8_append(q, k, v, cu_rows, cached, pos, theta, self._desc, *outs)
-        return outs
+        return _hxq.kv8_append(q, k, v, cu_rows, cached, pos, theta, self._desc, outs)
 
     def attend(self, q, k, v, cached, pos=None, theta=0.0, scale=None, weight=None, weight_out=None,
                out=None, out_dtype=None):
@@ -142,12 +128,9 @@ class HelixKV8Cache:
         (None: zeros) plus each block's share of the softmax summed over the query heads of its kv
         head; it may be weight.  Returns (out [batch, heads, D], weight_out); a sequence with a
         negative cached is skipped, its part of both not written.  One with no room left gives NaN."""
-        if out is None:
-            out = q.new_empty(q.shape, dtype=out_dtype)
-        _hxq.kv8_attn_decode(q, k, v, cached, pos, theta,
-                             q.shape[-1] ** -0.5 if scale is None else scale, self._desc, weight,
-                             weight_out, out)
-        return out, weight_out
+        return _hxq.kv8_attn_decode(q, k, v, cached, pos, theta,
+                                    q.shape[-1] ** -0.5 if scale is None else scale, self._desc,
+                                    weight, weight_out, out, out_dtype), weight_out
 
     def evict(self, weight, cached, keep, sink=0, recent=0):
         """Cut every sequence and head to `keep` full blocks (``kv8_evict``); the block table and
