@@ -45,6 +45,12 @@ __device__ __forceinline__ u32x2 lds_tr(const uint16_t *p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p)));
 }
 
+// 16 bytes a lane from `from` to LDS: lane l's to 16 l bytes behind `to` (the same in all lanes).
+__device__ __forceinline__ void load_lds16(const uint16_t *from, uint16_t *to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                     (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
 // Element offset of 16-byte chunk c of row r of a staged tile.  The chunk is XORed with the row's
 // low bits: rows 0..15 at one chunk (the reads of K) and rows r..r+3 at four neighbouring chunks
 // (the transposing reads of V) both hit distinct banks.
@@ -186,19 +192,22 @@ __device__ __forceinline__ void store_rows(const f32x16 (&o)[ND], float inv, uin
 //
 // NW = 4: 128 queries, one buffer, two blocks (at head_dim 64 three) on a compute unit.  NW = 8: 256
 // queries, two buffers and one barrier a step; half the bytes a query are staged.
+// KW: 32 queries a block, its four waves take steps of 64 keys in turn, each with a tile of its own in
+// LDS (loaded straight into it, no barrier), and join their sums at the end: for calls too small to fill
+// the chip, where the chain of a block's steps is the time.
 // SPLIT: blockIdx.y takes a part of the keys and leaves its sums for attn_join_kernel.
 //
 // Bound by the issue of MFMA, softmax and LDS reads together (of 1070 us the arithmetic of the softmax
 // is 14 %, the global loads 13 %, the LDS reads 10 %; the matrix pipe is busy half the time).  P in the
 // operands' 16 bits: half a step of each weight, of the size of the output's own rounding.  Measured:
 // 16 heads over 2, 16384 tokens 990 us (1.11 PFLOP/s); 28 over 4, twelve sequences of 371 to 2048 235;
-// fp16 at head_dim 64, six pieces over 7000 keys 106; 211 tokens 13.
-template <int NW, bool BF16, int D, bool CAUSAL, bool SPLIT>
+// fp16 at head_dim 64, six pieces over 7000 keys 103; 211 tokens 8.2 (KW).
+template <int NW, bool BF16, int D, bool CAUSAL, bool SPLIT, bool KW = false>
 __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArgs a) {
-    constexpr int THR = 64 * NW, BM = 32 * NW, NB = NW == 8 ? 2 : 1;
+    constexpr int THR = KW ? 64 : 64 * NW, BM = KW ? 32 : 32 * NW, NB = NW == 8 ? 2 : 1;
     constexpr int NK = D / 16, ND = D / 32, CPR = D / 8, NL = kBN * CPR / THR, RPP = THR / CPR;
     constexpr int ODD = BM / kBN + 3;    // steps in which some query does not see some key, at most
-    __shared__ __attribute__((aligned(16))) uint16_t sk[NB][kBN * D], sv[NB][kBN * D];
+    __shared__ __attribute__((aligned(16))) uint16_t sk[KW ? NW : NB][kBN * D], sv[KW ? NW : NB][kBN * D];
     __shared__ uint32_t odd[ODD][2];     // a bit for each of their keys
     // Blocks go round the 8 dies.  In large calls the heads of one kv head and tile stay on a die, and with
     // them the tiles of a kv head on as few as there are: their keys and values come from its L2 (28 heads
@@ -221,7 +230,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & 31, hh = lane >> 5;
     const int q_beg = at.q_beg, lq = at.lq, k_beg = at.k_beg, lk = at.lk;
-    const int i0 = at.tile * BM, iq = i0 + wave * 32 + ql;   // in the sequence
+    const int i0 = at.tile * BM, iq = i0 + (KW ? 0 : wave * 32) + ql;   // in the sequence
     const int past = lk - lq;
     const uint16_t *kp = static_cast<const uint16_t *>(a.k.p) + kvh * a.k.head + (int64_t)k_beg * a.k.row;
     const uint16_t *vp = static_cast<const uint16_t *>(a.v.p) + kvh * a.v.head + (int64_t)k_beg * a.v.row;
@@ -234,7 +243,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
     const int last = min(i0 + BM, lq) - 1;                              // the block's last query
     const int n_keys = keys_seen<CAUSAL>(last, lq, lk);
     const int lim = CAUSAL ? min(iq + past, lk - 1) : lk - 1;            // the lane's last key
-    const int lim_w = CAUSAL ? min(i0 + wave * 32 + 31 + past, lk - 1) : lk - 1;   // the most of the wave's
+    const int lim_w = CAUSAL ? min(i0 + (KW ? 0 : wave * 32) + 31 + past, lk - 1) : lk - 1;   // the most of the wave's
     const int lim_b = CAUSAL ? min(i0 + past, lk - 1) : lk - 1;          // the least of the block's
     const int steps = (n_keys + kBN - 1) / kBN, clean = max(min(n_keys, lim_b + 1), 0) / kBN & -NB;
     const int row_k = (ql & 0x13) | (ql & 4) << 1 | (ql & 8) >> 1;       // key of the lane's row
@@ -252,7 +261,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
 
     // a step's keys and values go through registers, asked for one step ahead
     u32x4 kr[NL], vr[NL];
-    const int tr = threadIdx.x / CPR, tc = threadIdx.x % CPR;
+    const int tr = (KW ? lane : threadIdx.x) / CPR, tc = (KW ? lane : threadIdx.x) % CPR;
     const uint32_t off_k = static_cast<uint32_t>(tr * a.k.row + tc * 8) * 2;
     const uint32_t off_v = static_cast<uint32_t>(tr * a.v.row + tc * 8) * 2;
     const auto fetch = [&](int t) {
@@ -301,11 +310,47 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
             *reinterpret_cast<u32x4 *>(sv[b] + swz<D>(tr + i * RPP, tc)) = vr[i];
         }
     };
+    // KW: a wave's own tile, straight into its place in LDS (a load's lanes write 1 KB in a row: lane l the
+    // chunk l % CPR of row l / CPR, so each asks for the chunk that belongs there)
+    const auto fetch_own = [&](const uint16_t *base, int64_t stride, int t, uint16_t *to) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int r = tr + i * RPP, c = (swz<D>(r, tc) - r * D) >> 3;
+            load_lds16(base + min(t * kBN + r, lk - 1) * stride + c * 8, to + i * RPP * D);
+        }
+    };
+    const auto drop_own = [&](int t, uint16_t *v) {
+        constexpr uint32_t ONE = BF16 ? 0x00800080u : 0x04000400u;   // carries into bit 15 of a half that is not finite
+        uint32_t any = 0u;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(v + swz<D>(tr + i * RPP, tc));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) any |= (w[e] & 0x7fff7fffu) + ONE;
+        }
+        if (!__any(any & 0x80008000u)) return;
+#pragma unroll 1
+        for (int i = 0; i < NL; ++i) {
+            const int r = tr + i * RPP;
+            u32x4 w = *reinterpret_cast<const u32x4 *>(v + swz<D>(r, tc));
+            bool found = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t x = w[e];
+                found |= drop_nonfinite<BF16>(x);
+                w[e] = x;
+            }
+            if (found) {
+                atomicOr(&odd[t - clean][r >> 5], 1u << (r & 31));
+                *reinterpret_cast<u32x4 *>(v + swz<D>(r, tc)) = w;
+            }
+        }
+    };
     // EDGE: some query of the block does not see some key of the step
     const auto compute = [&](int t, auto b_c, auto edge_c) {
         constexpr bool EDGE = decltype(edge_c)::value;
-        const uint16_t *k = sk[decltype(b_c)::value], *v = sv[decltype(b_c)::value];
-        if (EDGE && t * kBN > lim_w) return;   // nothing that the wave's queries see
+        const uint16_t *k = sk[KW ? wave : decltype(b_c)::value], *v = sv[KW ? wave : decltype(b_c)::value];
+        if (!KW && EDGE && t * kBN > lim_w) return;   // nothing that the wave's queries see
         f32x16 s[2];
         // the wave that multiplies goes before the one that is in its softmax
         __builtin_amdgcn_s_setprio(1);
@@ -386,7 +431,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
             lds_barrier();
         }
     };
-    if (t0 < t1) {
+    if (t0 < t1 && !KW) {
         fetch(t0);
         if constexpr (NB == 2) {
             lds_barrier();   // odd[] is cleared
@@ -396,18 +441,30 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
     }
     using B0 = std::integral_constant<int, 0>;
     using B1 = std::integral_constant<int, NB - 1>;
-    int t = t0;
-    for (; t < (SPLIT ? min(clean, t1) : clean); t += NB) {   // (with the min 3 % slower where it is not needed)
-        step(t, B0{}, std::false_type{});
-        if constexpr (NB == 2) step(t + 1, B1{}, std::false_type{});
-    }
-    for (; t < t1; t += NB) {
-        step(t, B0{}, std::true_type{});
-        if (NB == 2 && t + 1 < t1) step(t + 1, B1{}, std::true_type{});
+    if constexpr (KW) {
+        lds_barrier();   // odd[] is cleared
+        for (int t = t0 + wave; t < t1; t += NW) {
+            fetch_own(kp, a.k.row, t, sk[wave]);
+            fetch_own(vp, a.v.row, t, sv[wave]);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (t >= clean) drop_own(t, sv[wave]);
+            compute(t, B0{}, std::true_type{});
+        }
+    } else {
+        int t = t0;
+        for (; t < (SPLIT ? min(clean, t1) : clean); t += NB) {   // (with the min 3 % slower where it is not needed)
+            step(t, B0{}, std::false_type{});
+            if constexpr (NB == 2) step(t + 1, B1{}, std::false_type{});
+        }
+        for (; t < t1; t += NB) {
+            step(t, B0{}, std::true_type{});
+            if (NB == 2 && t + 1 < t1) step(t + 1, B1{}, std::true_type{});
+        }
     }
 
     __syncthreads();
     for (int t = max(clean, t0); t < t1; ++t) {
+        if (KW && (t - t0) % NW != wave) continue;
         uint64_t bits = odd[t - clean][0] | static_cast<uint64_t>(odd[t - clean][1]) << 32;
         for (; bits; bits &= bits - 1) {
             const int j = t * kBN + __builtin_ctzll(bits);
@@ -415,6 +472,49 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
         }
     }
     l = half_sum(l);
+    if constexpr (KW) {   // the waves' sums joined: a wave's in the place of its keys, chunks turned by the row
+        __shared__ float2 wml[NW][32];
+        float *so = reinterpret_cast<float *>(sk[wave]) + ql * D;
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+                *reinterpret_cast<f32x4 *>(so + 4 * ((8 * i + r / 2 + hh) ^ (ql & 15))) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+        if (hh == 0) wml[wave][ql] = float2{m * a.scale2, l};
+        __syncthreads();
+        const int j = threadIdx.x / 8, row = i0 + j;
+        if (row >= lq) return;
+        const bool sees = (CAUSAL ? min(row + past, lk - 1) : lk - 1) >= 0;
+        float mm = -INFINITY, ll = 0.f, f[NW], y[NW];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) mm = fmaxf(mm, wml[w][j].x);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            y[w] = wml[w][j].y;
+            f[w] = y[w] == 0.f ? 0.f : __builtin_amdgcn_exp2f(wml[w][j].x - mm);
+            ll = fmaf(f[w], y[w], ll);
+        }
+        const float inv = inv_sum(ll, sees);
+        const int64_t to = ((int64_t)(q_beg + row) * a.n_heads + head) * a.splits + blockIdx.y;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+            const int c = threadIdx.x % 8 + 8 * e;
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const f32x4 p = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(sk[w]) + j * D + 4 * (c ^ (j & 15)));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = fmaf(f[w], y[w] == 0.f ? 0.f : p[r], x[r]);
+            }
+            if constexpr (SPLIT)
+                *reinterpret_cast<f32x4 *>(a.part + to * D + 4 * c) = x;
+            else
+                *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + head * a.out_head + (int64_t)(q_beg + row) * a.out_row + 4 * c) =
+                    u32x2{pack16<BF16>(x[0] * inv, x[1] * inv), pack16<BF16>(x[2] * inv, x[3] * inv)};
+        }
+        if (SPLIT && threadIdx.x % 8 == 0) a.ml[to] = float2{mm, ll == 0.f && sees ? -0.f : ll};
+        return;
+    }
     if (iq >= lq) return;
     if constexpr (SPLIT) {
         const int64_t at = ((int64_t)(q_beg + iq) * a.n_heads + head) * a.splits + blockIdx.y;
@@ -480,32 +580,50 @@ using namespace hxq;
 namespace {
 
 struct PromptPlan {
-    int nw, splits;
+    int nw, bm, splits;
     int64_t part_bytes, bytes;   // workspace: part, then ml
 };
 
 // What depends on sizes that the host knows; lengths of sequences are on the device.
 PromptPlan prompt_plan(int64_t rows_q, int64_t rows_k, int64_t n_seqs, int64_t n_heads, int32_t D) {
-    PromptPlan p{4, 1, 0, 0};
+    PromptPlan p{4, 128, 1, 0, 0};
     // 8 waves for long sequences whose blocks reach every compute unit, 4 for the others (16 heads over 2,
     // us with 4 and 8 waves: one of 4096 tokens 136 and 124, of 8192 335 and 305, eight of 2048 178 and 173;
     // sixteen of 1024 116 and 123, one of 211 13 and 17): two blocks of 4 a unit hide each other's start,
     // 8 waves stage half the bytes.
     if (D == 128 && rows_q >= 1536 * n_seqs && rows_q / 256 * n_heads >= device_cu_count()) p.nw = 8;
-    if (p.nw == 8) return p;
-    // Few blocks: the keys of each are split, to as many blocks as run at once (two a compute unit, at
+    if (p.nw == 8) {
+        p.bm = 256;
+        return p;
+    }
+    const int64_t cus = device_cu_count(), held = (D == 64 ? 3 : 2) * cus;
+    const int64_t seqs = std::min(rows_q, n_seqs);
+    const int64_t keys = rows_k / seqs - rows_q / seqs / 2;   // that a query sees
+    // Small calls: a block takes 32 queries and its four waves different keys, so that its chain of steps is a
+    // quarter as long, and the keys are split while compute units idle.  It stages four times the bytes a query,
+    // so not past some keys a split; above one block a unit (head_dim 64: two and a half) it pays from some keys
+    // on.  us with 128 and 32 queries a block: 16 heads, a prompt of 211 13.2 and 8.2, of 512 20.7 and 10.8, of
+    // 1024 30.2 and 22.9, 8 queries over 2000 keys 14.8 and 10.7, 64 of a prompt 6.8 and 7.8; 28 heads, 600 24.0
+    // and 26.5, four of 100 10.1 and 15.2; at head_dim 64 512 12.3 and 7.4, two of 200 over 1200 16.2 and 11.4.
+    const int64_t small = std::max(seqs, (rows_q + 16 * seqs + 15) / 32) * n_heads;
+    if (rows_k / seqs > 96 && (small <= cus || (D == 64 ? 2 * small <= 5 * cus : small <= 2 * cus && keys >= 300))) {
+        const int64_t each = D == 64 ? 512 : 256;
+        const int64_t splits = std::max<int64_t>(1, std::min({cus / small, (keys + each - 1) / each, int64_t{kMaxSplits}}));
+        if (keys <= splits * (D == 64 ? 1600 : 1100)) {
+            p.bm = 32;
+            p.splits = static_cast<int>(splits);
+        }
+    }
+    // Few blocks of the others: the keys of each are split, to as many blocks as run at once (two a compute unit, at
     // head_dim 64 three), while a split keeps 192 keys (at head_dim 64 256, and 640 past one block a unit:
     // its steps are half the work).  16 heads, us with one block and split: 8 queries over 8000 keys 216
     // and 24, 512 over 8500 230 and 60, 2048 over 2048 61 and 51, 1000 over 1000 34 and 30; at head_dim 64
     // 2048 over 10000 137 and 115, 200 over 1200 22 and 18.
-    const int64_t cus = device_cu_count(), held = (D == 64 ? 3 : 2) * cus;
-    const int64_t seqs = std::min(rows_q, n_seqs);
     const int64_t blocks = std::max(seqs, (rows_q + 64 * seqs) / 128) * n_heads;
-    const int64_t keys = rows_k / seqs - rows_q / seqs / 2;   // that a query sees
     int64_t splits = std::max(std::min(cus / blocks, keys / 256), std::min(held / blocks, keys / (D == 64 ? 640 : 192)));
     // (one sequence: its blocks are alike, three splits take two rounds for three: 2304 over 3304 98 and 83)
     if (D == 128 && n_seqs == 1 && blocks > cus && blocks <= 2 * held / 3 && keys >= 3 * 512) splits = 3;
-    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)));
+    if (p.bm == 128) p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)));
     if (p.splits > 1) {
         p.part_bytes = rows_q * n_heads * p.splits * D * 4;
         p.bytes = p.part_bytes + rows_q * n_heads * p.splits * 8;
@@ -545,7 +663,7 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
     const PromptPlan plan = prompt_plan(rows_q, rows_k, n_seqs, n_heads, head_dim);
     HXQ_REQUIRE(plan.bytes == 0 || (workspace && workspace_bytes >= plan.bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "workspace too small or not 16-byte aligned");
-    const int64_t tiles = rows_q / (32 * plan.nw) + n_seqs;
+    const int64_t tiles = rows_q / plan.bm + n_seqs;
     // eight tiles of a kv head a die: below that some dies would go short (8 queries, 8192 keys, 16 heads: 50
     // us by die, 23 round)
     const bool by_die = tiles * n_kv_heads >= 64;
@@ -563,7 +681,8 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
         const auto by_c = [&](auto cc) {
             constexpr bool C = decltype(cc)::value;
             if (plan.splits > 1) {
-                hipLaunchKernelGGL((attn_prompt_kernel<4, B, D, C, true>), grid, dim3(256), 0, stream, a);
+                if (plan.bm == 32) hipLaunchKernelGGL((attn_prompt_kernel<4, B, D, C, true, true>), grid, dim3(256), 0, stream, a);
+                else hipLaunchKernelGGL((attn_prompt_kernel<4, B, D, C, true>), grid, dim3(256), 0, stream, a);
                 const auto joined = [&](auto ns) {
                     hipLaunchKernelGGL((attn_join_kernel<B, D, decltype(ns)::value>), join, dim3(256), 0, stream, a);
                 };
@@ -571,6 +690,10 @@ extern "C" int hxq_attn_prompt(const void *q, int64_t q_row_stride, int64_t q_he
                 else if (plan.splits <= 4) joined(std::integral_constant<int, 4>{});
                 else if (plan.splits <= 8) joined(std::integral_constant<int, 8>{});
                 else joined(std::integral_constant<int, kMaxSplits>{});
+                return;
+            }
+            if (plan.bm == 32) {
+                hipLaunchKernelGGL((attn_prompt_kernel<4, B, D, C, false, true>), grid, dim3(256), 0, stream, a);
                 return;
             }
             if constexpr (D == 128)

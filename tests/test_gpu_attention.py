@@ -222,6 +222,30 @@ def test_prompt_scores_of_minus_infinity(dev, dt, lens, past, heads, bad):
         assert ((got[rq] - out).abs() <= tol)[~none].all()
 
 
+@pytest.mark.parametrize("dt,heads,D,lens,past", [
+    (BF, 4, 128, [5], [2000]), (FP, 4, 64, [40], [900]),       # waves with keys of their own, split or not
+    (BF, 64, 128, [100], [6000]), (FP, 64, 64, [100], [9000])])  # blocks of 128 queries, split
+def test_prompt_split_unseen_values(dev, dt, heads, D, lens, past):
+    """Values that are not finite in the last rows, which the first queries do not see, and keys too."""
+    q, k, v, cu, cu_k = _prompt_case(lens, heads, 2, D, dt, 41, past)
+    n = len(k)
+    v[n - 1, 0, 1], v[n - 3, 0, 7], v[n - 4, 1, 2] = math.nan, math.inf, -math.inf
+    k[n - 2, 1, 5] = math.nan
+    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu_k.to(dev)).cpu()
+    h = heads // 2
+    assert got[-1, :h, 1].isnan().all() and got[:-1, :h, 1].isfinite().all()
+    assert not got[-3:, :h, 7].isfinite().any() and got[:-3, :h, 7].isfinite().all()
+    assert got[-2:, h:].isnan().all() and got[:-4, h:].isfinite().all()
+    assert not got[-4:, h:, 2].isfinite().any()
+    v[n - 1, 0, 1] = v[n - 3, 0, 7] = v[n - 4, 1, 2] = 0
+    k[n - 2, 1, 5] = 0
+    got[-1, :h, 1] = got[-3:, :h, 7] = got[-4:, h:] = 0
+    want = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu_k.to(dev)).cpu()
+    _check_prompt(want, q, k, v, cu, cu_k)
+    want[-1, :h, 1] = want[-3:, :h, 7] = want[-4:, h:] = 0
+    assert torch.equal(got, want)
+
+
 def test_prompt_neighbours_and_rows_behind(dev):
     """NaN in rows of no sequence reach nobody; their rows of out stay as they were."""
     q, k, v, cu, _ = _prompt_case([70, 60], 4, 2, 64, BF, 7)
