@@ -19,8 +19,8 @@ struct PromptArgs {
 
 constexpr int kMaxSplits = 16;
 
-// Steps of 64 keys of one split; at least 4.
-__device__ __forceinline__ int steps_per_split(int steps, int splits) { return max((steps + splits - 1) / splits, 4); }
+// Steps of 64 keys of one split; at least 4, and even (steps are taken in pairs).
+__device__ __forceinline__ int steps_per_split(int steps, int splits) { return max((steps + splits - 1) / splits + 1 & ~1, 4); }
 
 // Keys that the queries up to `last` of a sequence see.
 template <bool CAUSAL>
@@ -190,8 +190,10 @@ __device__ __forceinline__ void store_rows(const f32x16 (&o)[ND], float inv, uin
 // does not see some key, such values are staged as 0, their rows marked, and added at the end to the
 // queries that see them.
 //
-// NW = 4: 128 queries, one buffer, two blocks (at head_dim 64 three) on a compute unit.  NW = 8: 256
-// queries, two buffers and one barrier a step; half the bytes a query are staged.
+// NW = 4: 128 queries, two blocks on a compute unit, two buffers that the next step's loads fill directly
+// (twelve sequences 226 us, one buffer filled through registers 240); at head_dim 64 three blocks, one
+// buffer, through registers (101 us; as above 106).  NW = 8: 256 queries, two buffers, through registers
+// (992 us; directly 1003); half the bytes a query are staged.
 // KW: 32 queries a block, its four waves take steps of 64 keys in turn, each with a tile of its own in
 // LDS (loaded straight into it, no barrier), and join their sums at the end: for calls too small to fill
 // the chip, where the chain of a block's steps is the time.
@@ -200,11 +202,12 @@ __device__ __forceinline__ void store_rows(const f32x16 (&o)[ND], float inv, uin
 // Bound by the issue of MFMA, softmax and LDS reads together (of 1070 us the arithmetic of the softmax
 // is 14 %, the global loads 13 %, the LDS reads 10 %; the matrix pipe is busy half the time).  P in the
 // operands' 16 bits: half a step of each weight, of the size of the output's own rounding.  Measured:
-// 16 heads over 2, 16384 tokens 990 us (1.11 PFLOP/s); 28 over 4, twelve sequences of 371 to 2048 235;
+// 16 heads over 2, 16384 tokens 990 us (1.11 PFLOP/s); 28 over 4, twelve sequences of 371 to 2048 223;
 // fp16 at head_dim 64, six pieces over 7000 keys 103; 211 tokens 8.2 (KW).
 template <int NW, bool BF16, int D, bool CAUSAL, bool SPLIT, bool KW = false>
 __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArgs a) {
-    constexpr int THR = KW ? 64 : 64 * NW, BM = KW ? 32 : 32 * NW, NB = NW == 8 ? 2 : 1;
+    constexpr int THR = KW ? 64 : 64 * NW, BM = KW ? 32 : 32 * NW, NB = KW || D == 64 ? 1 : 2;
+    constexpr bool STAGED = NW == 8 || !KW && D == 64;     // through registers
     constexpr int NK = D / 16, ND = D / 32, CPR = D / 8, NL = kBN * CPR / THR, RPP = THR / CPR;
     constexpr int ODD = BM / kBN + 3;    // steps in which some query does not see some key, at most
     __shared__ __attribute__((aligned(16))) uint16_t sk[KW ? NW : NB][kBN * D], sv[KW ? NW : NB][kBN * D];
@@ -259,11 +262,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
     }
     if (threadIdx.x < 2 * ODD) odd[threadIdx.x >> 1][threadIdx.x & 1] = 0u;
 
-    // a step's keys and values go through registers, asked for one step ahead
+    // a step's keys and values, asked for one step ahead
     u32x4 kr[NL], vr[NL];
     const int tr = (KW ? lane : threadIdx.x) / CPR, tc = (KW ? lane : threadIdx.x) % CPR;
-    const uint32_t off_k = static_cast<uint32_t>(tr * a.k.row + tc * 8) * 2;
-    const uint32_t off_v = static_cast<uint32_t>(tr * a.v.row + tc * 8) * 2;
+    const int first = !STAGED ? swz<D>(tr, tc) - tr * D : tc * 8;   // in its row
+    const uint32_t off_k = static_cast<uint32_t>(tr * a.k.row + first) * 2;
+    const uint32_t off_v = static_cast<uint32_t>(tr * a.v.row + first) * 2;
     const auto fetch = [&](int t) {
         const char *kb = reinterpret_cast<const char *>(kp + t * kBN * a.k.row);
         const char *vb = reinterpret_cast<const char *>(vp + t * kBN * a.v.row);
@@ -310,16 +314,27 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
             *reinterpret_cast<u32x4 *>(sv[b] + swz<D>(tr + i * RPP, tc)) = vr[i];
         }
     };
-    // KW: a wave's own tile, straight into its place in LDS (a load's lanes write 1 KB in a row: lane l the
-    // chunk l % CPR of row l / CPR, so each asks for the chunk that belongs there)
-    const auto fetch_own = [&](const uint16_t *base, int64_t stride, int t, uint16_t *to) {
+    // A tile straight into LDS (a load's lanes write 1 KB in a row: a lane has chunk tc of its row, so it asks
+    // for the chunk that belongs there).
+    const int tile_at = KW ? 0 : wave * (64 / CPR) * D;
+    const auto fetch_lds = [&](const uint16_t *base, int64_t stride, uint32_t off, int t, uint16_t *to) {
+        if (!KW && (t + 1) * kBN <= lk) {   // (RPP is a multiple of 16: the same chunk in all rows of a thread)
+            const char *b = reinterpret_cast<const char *>(base + t * kBN * stride);
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
+            for (int i = 0; i < NL; ++i)
+                load_lds16(reinterpret_cast<const uint16_t *>(b + i * RPP * stride * 2 + off), to + tile_at + i * RPP * D);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {   // rows behind the last are the last again: no query sees them
             const int r = tr + i * RPP, c = (swz<D>(r, tc) - r * D) >> 3;
-            load_lds16(base + min(t * kBN + r, lk - 1) * stride + c * 8, to + i * RPP * D);
+            load_lds16(base + min(t * kBN + r, lk - 1) * stride + c * 8, to + tile_at + i * RPP * D);
         }
     };
-    const auto drop_own = [&](int t, uint16_t *v) {
+    // Waits for the thread's own part of a tile and takes what is not finite out of its values.
+    const auto take_lds = [&](int t, uint16_t *v) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (t < clean) return;
         constexpr uint32_t ONE = BF16 ? 0x00800080u : 0x04000400u;   // carries into bit 15 of a half that is not finite
         uint32_t any = 0u;
 #pragma unroll
@@ -419,23 +434,39 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
         }
     };
     const auto step = [&](int t, auto b_c, auto edge_c) {
+        constexpr int other = decltype(b_c)::value ^ 1;
+        const bool more = t + 1 < t1;
         if constexpr (NB == 1) {
             lds_barrier();
             put(t, 0);
             lds_barrier();
         }
-        if (t + 1 < t1) fetch(t + 1);
+        if constexpr (STAGED) {
+            if (more) fetch(t + 1);
+        } else if (more) {
+            fetch_lds(kp, a.k.row, off_k, t + 1, sk[other]);
+            fetch_lds(vp, a.v.row, off_v, t + 1, sv[other]);
+        }
         compute(t, b_c, edge_c);
         if constexpr (NB == 2) {
-            if (t + 1 < t1) put(t + 1, decltype(b_c)::value ^ 1);
+            if (more) {
+                if constexpr (STAGED) put(t + 1, other);
+                else take_lds(t + 1, sv[other]);
+            }
             lds_barrier();
         }
     };
     if (t0 < t1 && !KW) {
-        fetch(t0);
+        if constexpr (STAGED) {
+            fetch(t0);
+        } else {
+            fetch_lds(kp, a.k.row, off_k, t0, sk[0]);
+            fetch_lds(vp, a.v.row, off_v, t0, sv[0]);
+        }
         if constexpr (NB == 2) {
             lds_barrier();   // odd[] is cleared
-            put(0, 0);
+            if constexpr (STAGED) put(t0, 0);
+            else take_lds(t0, sv[0]);
             lds_barrier();
         }
     }
@@ -444,10 +475,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
     if constexpr (KW) {
         lds_barrier();   // odd[] is cleared
         for (int t = t0 + wave; t < t1; t += NW) {
-            fetch_own(kp, a.k.row, t, sk[wave]);
-            fetch_own(vp, a.v.row, t, sv[wave]);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (t >= clean) drop_own(t, sv[wave]);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the last step's reads are done
+            fetch_lds(kp, a.k.row, off_k, t, sk[wave]);
+            fetch_lds(vp, a.v.row, off_v, t, sv[wave]);
+            take_lds(t, sv[wave]);
             compute(t, B0{}, std::true_type{});
         }
     } else {
@@ -587,18 +618,18 @@ struct PromptPlan {
 // What depends on sizes that the host knows; lengths of sequences are on the device.
 PromptPlan prompt_plan(int64_t rows_q, int64_t rows_k, int64_t n_seqs, int64_t n_heads, int32_t D) {
     PromptPlan p{4, 128, 1, 0, 0};
-    // 8 waves for long sequences whose blocks reach every compute unit, 4 for the others (16 heads over 2,
-    // us with 4 and 8 waves: one of 4096 tokens 136 and 124, of 8192 335 and 305, eight of 2048 178 and 173;
-    // sixteen of 1024 116 and 123, one of 211 13 and 17): two blocks of 4 a unit hide each other's start,
-    // 8 waves stage half the bytes.
-    if (D == 128 && rows_q >= 1536 * n_seqs && rows_q / 256 * n_heads >= device_cu_count()) p.nw = 8;
+    const int64_t cus = device_cu_count(), held = (D == 64 ? 3 : 2) * cus;
+    const int64_t seqs = std::min(rows_q, n_seqs);
+    const int64_t keys = rows_k / seqs - rows_q / seqs / 2;   // that a query sees
+    // 8 waves where queries see many keys and there are two blocks a compute unit, 4 for the others (16 heads
+    // over 2, us with 4 and 8 waves: one of 16384 tokens 1063 and 1023, of 8192 292 and 272, of 4096 106 and 120,
+    // eight of 2048 164 and 174, four of 2048 behind 4000 336 and 329): two blocks of 4 a unit hide each other's
+    // start, 8 waves stage half the bytes.
+    if (D == 128 && keys >= 4096 && rows_q / 256 * n_heads >= 2 * cus) p.nw = 8;
     if (p.nw == 8) {
         p.bm = 256;
         return p;
     }
-    const int64_t cus = device_cu_count(), held = (D == 64 ? 3 : 2) * cus;
-    const int64_t seqs = std::min(rows_q, n_seqs);
-    const int64_t keys = rows_k / seqs - rows_q / seqs / 2;   // that a query sees
     // Small calls: a block takes 32 queries and its four waves different keys, so that its chain of steps is a
     // quarter as long, and the keys are split while compute units idle.  It stages four times the bytes a query,
     // so not past some keys a split; above one block a unit (head_dim 64: two and a half) it pays from some keys

@@ -65,11 +65,11 @@ def test_prompt(dev, dt, heads, kv, D, lens):
     _check_prompt(got, q, k, v, cu, cu)
 
 
-def _behind(q, n_seqs):
-    """q with rows of no sequence behind it, to 1600 rows a sequence: a large call, which the 8-wave
-    blocks take (from 64 heads on)."""
-    more = torch.full((max(1600 * n_seqs - q.shape[0], 0), *q.shape[1:]), math.nan, dtype=q.dtype)
-    return torch.cat([q, more])
+def _behind(x, rows):
+    """x with rows of no sequence behind it.  2100 rows of q and 5200 of k and v a sequence make a large
+    call, which the 8-wave blocks take (from 64 heads on)."""
+    more = torch.full((max(rows - x.shape[0], 0), *x.shape[1:]), math.nan, dtype=x.dtype)
+    return torch.cat([x, more])
 
 
 @pytest.mark.parametrize("causal", [True, False])
@@ -80,8 +80,12 @@ def _behind(q, n_seqs):
 def test_prompt_with_many_heads(dev, dt, D, lens, past, causal, large):
     """Many heads over ragged sequences, keys before and fewer keys than queries; both block sizes."""
     q, k, v, cu, cu_k = _prompt_case(lens, 64, 8, D, dt, 10, [max(p, -n) for p, n in zip(past, lens)])
-    got = attn_prompt((_behind(q, len(lens)) if large else q).to(dev), k.to(dev), v.to(dev), cu.to(dev),
-                      cu_k.to(dev), causal=causal)[:q.shape[0]]
+    qq, kk, vv = q, k, v
+    if large:
+        n = len(lens)
+        qq, kk, vv = _behind(q, 2100 * n), _behind(k, 5200 * n), _behind(v, 5200 * n)
+    got = attn_prompt(qq.to(dev), kk.to(dev), vv.to(dev), cu.to(dev), cu_k.to(dev),
+                      causal=causal)[:q.shape[0]]
     _check_prompt(got, q, k, v, cu, cu_k, causal=causal)
 
 
@@ -170,11 +174,12 @@ def test_prompt_scores_that_grow(dev):
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("lens", [[200], [70, 130]])
-@pytest.mark.parametrize("heads", [4, 64])
-def test_prompt_unseen_values_have_no_influence(dev, bad, lens, heads):
+@pytest.mark.parametrize("heads,large", [(4, False), (64, False), (64, True)])
+def test_prompt_unseen_values_have_no_influence(dev, bad, lens, heads, large):
     q, k, v, cu, _ = _prompt_case(lens, heads, 2, 128, BF, 6)
-    if heads == 64:
-        q = _behind(q, len(lens))
+    if large:
+        n = len(lens)
+        q, k, v = _behind(q, 2100 * n), _behind(k, 5200 * n), _behind(v, 5200 * n)
     for t in (3, 40, 64, 101, 127, 199):
         v[t, 0, 5] = bad
         k[t, 1, 9] = math.nan
