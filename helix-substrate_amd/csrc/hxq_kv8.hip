@@ -861,7 +861,7 @@ __global__ __launch_bounds__(kEvThr) void kv8_evict_kernel(const float *weight, 
         }
     }
     const int stay = cut ? keep : full;
-    int n_kept = 0, n_tie = 0;     // of the blocks before this round's
+    int n_kept = 0, n_tie = 0;     // of the blocks before this pass's
     for (int j0 = 0; j0 < n_blocks; j0 += kEvThr) {
         const int j = j0 + tid;
         const bool in = j < full, fixed = in && (!cut || j < sink || j >= full - recent);

@@ -545,8 +545,8 @@ int hxq_argmax(const float *logits, int64_t n, int32_t *out_id, int32_t *pos,
  * are fp32, the softmax weights are rounded to dtype before the product with v.  Rows of out that
  * belong to no sequence are left as they were; offsets are clamped to [0, rows_q] and [0, rows_k].
  * scale: 2^-100 to 2^100.  Row strides of k and v: 0 to 2^24 - 1 elements.  out may be q, and must
- * not overlap k or v.  workspace: device scratch of hxq_attn_prompt_workspace_bytes(...) bytes (0 but
- * for few queries over many keys), written and read within the call.
+ * not overlap k or v.  workspace: device scratch of hxq_attn_prompt_workspace_bytes(...) bytes (0 in
+ * large calls; in others the keys may be split), written and read within the call.
  */
 int64_t hxq_attn_prompt_workspace_bytes(int64_t rows_q, int64_t rows_k, int32_t n_seqs,
                                         int32_t n_heads, int32_t head_dim);
