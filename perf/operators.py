@@ -10,7 +10,6 @@ v_tail [batch, n_kv, D, 64]) and a table of each sequence's and head's blocks in
 """
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -235,7 +234,6 @@ def prepare(case, seed):
 
 
 # --- the framework's calls ------------------------------------------------------------------------
-@functools.lru_cache(maxsize=1)
 def _kernels():
     pkg = str(Path(__file__).resolve().parents[1] / "helix-substrate_amd")
     if pkg not in sys.path:
