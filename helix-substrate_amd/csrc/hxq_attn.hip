@@ -497,6 +497,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
     for (int t = max(clean, t0); t < t1; ++t) {
         if (KW && (t - t0) % NW != wave) continue;
         uint64_t bits = odd[t - clean][0] | static_cast<uint64_t>(odd[t - clean][1]) << 32;
+        if (lk - t * kBN < kBN) bits &= (1ull << (lk - t * kBN)) - 1;   // rows behind the last were staged as the last
         for (; bits; bits &= bits - 1) {
             const int j = t * kBN + __builtin_ctzll(bits);
             add_odd<BF16, ND>(vp + (int64_t)j * a.v.row + 4 * hh, j <= lim, o);
