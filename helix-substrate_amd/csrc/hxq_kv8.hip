@@ -826,7 +826,8 @@ __global__ __launch_bounds__(kEvThr) void kv8_evict_kernel(const float *weight, 
     __shared__ int s_left, wsum[2][kEvThr / kWave];
     const int64_t base = (int64_t)blockIdx.x * n_blocks;
     const int b = blockIdx.x / n_kv, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n = cached[b], full = n < 0 ? 0 : min(n / kBlk, n_blocks);
+    // tokens past the cache were never stored: they do not come back when there is room again
+    const int n = min(cached[b], n_blocks * kBlk), full = n < 0 ? 0 : n / kBlk;
     const float *w = weight + base;
     const bool cut = full > keep;
     uint32_t key = 0;      // bits of the least key that stays, and how many of that key stay

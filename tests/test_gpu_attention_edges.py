@@ -7,9 +7,8 @@ import pytest
 import torch
 
 import attention_ref as ref
-from helix_substrate import _hxq
-from helix_substrate.attention import attn_prompt
-from test_gpu_attention import BF, FP, _check_prompt, _prompt_case
+from helix_substrate.attention import BLOCK, HelixKV8Cache, attn_prompt, kv8_evict
+from test_gpu_attention import (BF, F32, FP, _check_attend, _cpu, _gen, _i32, _prompt_case, _rows)
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +43,44 @@ def test_prompt_values_that_are_not_finite_in_the_last_row(dev, dt, heads, kv, D
     got[first:, :group, 3] = want[first:, :group, 3] = 0
     got[first:, :group, D - 1] = want[first:, :group, D - 1] = 0
     assert torch.equal(got, want)
+
+
+# --- eviction ------------------------------------------------------------------------------------------
+def _cut(x, heads, kv):
+    return x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
+
+
+@pytest.mark.parametrize("n_blocks,cached,keep", [
+    (2, [128 + 12, 128, 2 * 128 + 3], 1), (2, [128 + 5, 64, 3 * 64 + 3], 2),
+    (9, [9 * 64 + 5, 10 * 64 + 3, 64], 4), (1100, [1100 * 64 + 63, 2 ** 31 - 1, 5], 7)])
+def test_evict_counts_past_the_cache(dev, n_blocks, cached, keep):
+    """Tokens past the cache were never stored: the count that comes out names stored ones only."""
+    g = _gen(51)
+    w = torch.randn(3, 2, n_blocks, generator=g)
+    blocks = torch.stack([torch.randperm(n_blocks, generator=g) for _ in range(6)]).view(3, 2, -1).to(torch.int32)
+    cnt = torch.tensor(cached, dtype=torch.int32)
+    got = kv8_evict(w.to(dev), blocks.to(dev), cnt.to(dev), keep)
+    want = ref.evict(w, blocks, cnt.clamp(max=n_blocks * BLOCK), keep, 0, 0)
+    for a, b in zip(got, want):
+        assert torch.equal(a.cpu(), b)
+
+
+def test_evict_after_a_prompt_that_had_no_room(dev):
+    """128 tokens of 140 fit; after eviction a token sees the block that stayed and itself."""
+    heads, kv, D = 4, 2, 64
+    cache = HelixKV8Cache.empty(1, kv, D, 128, device=dev)
+    x = _rows(140, heads, kv, D, BF, 52).to(dev)
+    cached, w = _i32([0], dev), cache.new_weight()
+    for a, b in ((0, 100), (100, 140)):
+        cache.append(*_cut(x[a:b], heads, kv), cached, _i32([0, b - a], dev), theta=1e6)
+        cached += b - a
+    t = _rows(1, heads, kv, D, F32, 53)
+    out, _ = cache.attend(*_cut(t.to(dev), heads, kv), cached, theta=1e6, weight=w, weight_out=w)
+    assert out.isnan().all() and (w == 0).all()
+    cached = cache.evict(w, cached, keep=1)
+    assert int(cached) == 64
+    before = _cpu(cache)
+    out, _ = cache.attend(*_cut(t.to(dev), heads, kv), cached, pos=_i32([140], dev), theta=1e6, out_dtype=F32)
+    now = _cpu(cache)
+    before.k_tail[:, :, 0], before.v_tail[..., 0] = now.k_tail[:, :, 0], now.v_tail[..., 0]
+    _check_attend(before, t, heads, [64], [140], out, None, 1e6, F32)
