@@ -237,10 +237,10 @@ class HelixDecoder:
                     w.zero_()
 
     def prefill(self, prompt_ids):
-        """Feed the prompt token by token (teacher forced); leaves the greedy
-        successor of the last prompt token in self.tok."""
+        """Feed the prompt token by token (teacher forced) behind what the caches hold; leaves the
+        greedy successor of the last prompt token in self.tok."""
         ids = torch.as_tensor(prompt_ids, dtype=torch.int32, device=self.device)
-        if ids.numel() >= self.cfg.max_seq:
+        if ids.numel() >= self.cfg.max_seq or self._cached() + ids.numel() > self.cfg.max_seq:
             raise ValueError("prompt longer than max_seq")
         for t in range(ids.numel()):
             self.tok.copy_(ids[t:t + 1])
