@@ -827,8 +827,16 @@ __global__ __launch_bounds__(kEvThr) void kv8_evict_kernel(const float *weight, 
     const int64_t base = (int64_t)blockIdx.x * n_blocks;
     const int b = blockIdx.x / n_kv, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // tokens past the cache were never stored: they do not come back when there is room again
-    const int n = min(cached[b], n_blocks * kBlk), full = n < 0 ? 0 : n / kBlk;
+    const int n = min(cached[b], n_blocks * kBlk), full = n / kBlk;
     const float *w = weight + base;
+    if (n < 0) {   // skipped: its blocks and weights as they are
+        for (int j = tid; j < n_blocks; j += kEvThr) {
+            b_out[base + j] = blocks ? blocks[base + j] : j;
+            w_out[base + j] = w[j];
+        }
+        if (tid == 0 && blockIdx.x % n_kv == 0) c_out[b] = n;
+        return;
+    }
     const bool cut = full > keep;
     uint32_t key = 0;      // bits of the least key that stays, and how many of that key stay
     int left = keep - sink - recent;
@@ -902,7 +910,7 @@ __global__ __launch_bounds__(kEvThr) void kv8_evict_kernel(const float *weight, 
     }
     if (tid == 0) {
         if (full < n_blocks) w_out[base + stay] = w[full];   // the unfinished block's
-        if (blockIdx.x % n_kv == 0) c_out[b] = n < 0 ? n : n - (full - stay) * kBlk;
+        if (blockIdx.x % n_kv == 0) c_out[b] = n - (full - stay) * kBlk;
     }
 }
 

@@ -639,8 +639,9 @@ int hxq_kv8_attn_decode(const void *q, int64_t q_row_stride, int64_t q_head_stri
  * the lowest index; NaN counts as the greatest).  No cache data moves: blocks_out [batch,
  * n_kv_heads, n_blocks] holds the blocks that stay in their order, then the others; weight_out the
  * weights likewise, the unfinished block's behind those that stay, zero from there on; cached_out
- * the new counts.  A count past n_blocks * 64 is taken as n_blocks * 64: tokens past the cache were not
- * stored.  Outputs must not be the inputs.  blocks_in NULL = 0, 1, 2, ...
+ * the new counts.  A count past n_blocks * 64 is taken as n_blocks * 64: tokens past the cache were
+ * not stored.  Of a skipped sequence (cached < 0) the outputs are copies of the inputs.  Outputs must
+ * not be the inputs.  blocks_in NULL = 0, 1, 2, ...
  */
 int hxq_kv8_evict(const float *weight, const int32_t *blocks_in, const int32_t *cached,
                   int32_t batch, int32_t n_kv_heads, int32_t n_blocks, int32_t keep, int32_t sink,

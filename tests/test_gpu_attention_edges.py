@@ -84,3 +84,18 @@ def test_evict_after_a_prompt_that_had_no_room(dev):
     now = _cpu(cache)
     before.k_tail[:, :, 0], before.v_tail[..., 0] = now.k_tail[:, :, 0], now.v_tail[..., 0]
     _check_attend(before, t, heads, [64], [140], out, None, 1e6, F32)
+
+
+@pytest.mark.parametrize("n_blocks", [1, 9, 1500])
+def test_evict_leaves_skipped_sequences(dev, n_blocks):
+    """A negative count skips a sequence: its blocks, weights and count come out as they were."""
+    g = _gen(54)
+    w = torch.rand(3, 2, n_blocks, generator=g)
+    blocks = torch.stack([torch.randperm(n_blocks, generator=g) for _ in range(6)]).view(3, 2, -1).to(torch.int32)
+    cnt = torch.tensor([-1, 64 * n_blocks, -(2 ** 31)], dtype=torch.int32)
+    got = [t.cpu() for t in kv8_evict(w.to(dev), blocks.to(dev), cnt.to(dev), 1)]
+    want = ref.evict(w[1:2], blocks[1:2], cnt[1:2], 1, 0, 0)
+    for out, src, one in zip(got, (blocks, w, cnt), want):
+        assert torch.equal(out[[0, 2]], src[[0, 2]]) and torch.equal(out[1:2], one)
+    order = kv8_evict(w.to(dev), None, cnt.to(dev), 1)[0].cpu()
+    assert torch.equal(order[[0, 2]], torch.arange(n_blocks, dtype=torch.int32).expand(2, 2, -1))
