@@ -17,6 +17,8 @@ and positions are int32 on the device, so that nothing waits for the host.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _hxq
@@ -146,7 +148,7 @@ class HelixKV8Cache:
     def read(self, seq, cached):
         """Keys and values of one sequence's first `cached` tokens (a host number) in 16 bits,
         [cached, n_kv, D] each: what a prompt that continues them passes to `attn_prompt` before its
-        own rows.  Exact in bf16."""
+        own rows.  Exact in bf16.  A block that the table places outside the cache reads as NaN."""
         n, held = divmod(int(cached), BLOCK)
         n_kv, n_blocks, _, D = self.k.shape[1:]
         if not 0 <= int(cached) <= self.max_tokens:
@@ -154,12 +156,14 @@ class HelixKV8Cache:
         at = torch.arange(n, device=self.k.device).expand(n_kv, n)
         if self.blocks is not None:
             at = self.blocks[seq, :, :n].long()
+        known = (at >= 0) & (at < n_blocks)
+        at = at.where(known, 0)
         h = torch.arange(n_kv, device=self.k.device)[:, None]
         out = []
         for x8, scale, tail, turn in ((self.k, self.k_scale, self.k_tail, False),
                                       (self.v, self.v_scale, self.v_tail, True)):
             x = x8[seq].view(torch.uint8)[h, at].view(torch.float8_e4m3fn).float()
-            x = (x * scale[seq][h, at][..., None, None]).to(self.dtype)
+            x = (x * scale[seq][h, at].where(known, math.nan)[..., None, None]).to(self.dtype)
             last = tail[seq]
             if turn:
                 x, last = x.transpose(-1, -2), last.transpose(-1, -2)

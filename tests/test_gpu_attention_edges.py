@@ -99,3 +99,18 @@ def test_evict_leaves_skipped_sequences(dev, n_blocks):
         assert torch.equal(out[[0, 2]], src[[0, 2]]) and torch.equal(out[1:2], one)
     order = kv8_evict(w.to(dev), None, cnt.to(dev), 1)[0].cpu()
     assert torch.equal(order[[0, 2]], torch.arange(n_blocks, dtype=torch.int32).expand(2, 2, -1))
+
+
+# --- what a cache holds, in 16 bits ----------------------------------------------------------------------
+@pytest.mark.parametrize("entry", [-1, 4, 2 ** 31 - 1, -(2 ** 31)])
+def test_read_of_blocks_that_the_table_does_not_place(dev, entry):
+    """An entry outside the cache reads as NaN, as `attend` takes it; the other heads as they were."""
+    kv, D, n = 2, 64, 150
+    cache = HelixKV8Cache.empty(2, kv, D, 4 * BLOCK, device=dev)
+    x = _rows(2 * n, 0, kv, D, BF, 61).to(dev)
+    cache.append(None, *_cut(x, 0, kv)[1:], _i32([0, 0], dev), _i32([0, n, 2 * n], dev))
+    want = cache.read(1, n)
+    cache.blocks[1, 1, 0] = entry
+    for got, was in zip(cache.read(1, n), want):
+        assert got[:BLOCK, 1].isnan().all()
+        assert torch.equal(got[BLOCK:], was[BLOCK:]) and torch.equal(got[:, 0], was[:, 0])
