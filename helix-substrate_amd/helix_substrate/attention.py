@@ -148,7 +148,8 @@ class HelixKV8Cache:
     def read(self, seq, cached):
         """Keys and values of one sequence's first `cached` tokens (a host number) in 16 bits,
         [cached, n_kv, D] each: what a prompt that continues them passes to `attn_prompt` before its
-        own rows.  Exact in bf16.  A block that the table places outside the cache reads as NaN."""
+        own rows.  Exact in bf16; in fp16 up to its greatest value.  A block that the table places
+        outside the cache reads as NaN."""
         n, held = divmod(int(cached), BLOCK)
         n_kv, n_blocks, _, D = self.k.shape[1:]
         if not 0 <= int(cached) <= self.max_tokens:
@@ -163,7 +164,10 @@ class HelixKV8Cache:
         for x8, scale, tail, turn in ((self.k, self.k_scale, self.k_tail, False),
                                       (self.v, self.v_scale, self.v_tail, True)):
             x = x8[seq].view(torch.uint8)[h, at].view(torch.float8_e4m3fn).float()
-            x = (x * scale[seq][h, at].where(known, math.nan)[..., None, None]).to(self.dtype)
+            x = x * scale[seq][h, at].where(known, math.nan)[..., None, None]
+            if self.dtype == torch.float16:   # 63488 to 65504 were stored as 65536
+                x = x.clamp(-65504, 65504)
+            x = x.to(self.dtype)
             last = tail[seq]
             if turn:
                 x, last = x.transpose(-1, -2), last.transpose(-1, -2)

@@ -114,3 +114,17 @@ def test_read_of_blocks_that_the_table_does_not_place(dev, entry):
     for got, was in zip(cache.read(1, n), want):
         assert got[:BLOCK, 1].isnan().all()
         assert torch.equal(got[BLOCK:], was[BLOCK:]) and torch.equal(got[:, 0], was[:, 0])
+
+
+def test_read_next_to_the_end_of_fp16(dev):
+    """63488 lies half way between the e4m3 values 240 and 256 times 256 and goes to the even one, 65536,
+    which fp16 does not hold: it reads as 65504, not as infinity.  NaN stays NaN."""
+    D, ends = 64, [65504.0, -65504.0, 63488.0, -63488.0, 63456.0]
+    x = torch.zeros(BLOCK, 1, D, dtype=FP)
+    x[0, 0, :5] = torch.tensor(ends, dtype=FP)
+    x[1, 0, 0] = math.nan
+    cache = HelixKV8Cache.empty(1, 1, D, 2 * BLOCK, dtype=FP, device=dev)
+    cache.append(None, x.to(dev), x.to(dev), _i32([0], dev), _i32([0, BLOCK], dev))
+    for got in cache.read(0, BLOCK):
+        assert got[0, 0, :5].tolist() == [65504.0, -65504.0, 65504.0, -65504.0, 61440.0]
+        assert got[1, 0, 0].isnan() and (got[2:] == 0).all()
