@@ -402,14 +402,18 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArg
             const float mn = fmaxf(m, mx);
             const float al = m == mn ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.scale2);   // both may be -inf
             m = mn;
-            keep = m + 8.f / a.scale2;
+            keep = BF16 || fabsf(m * a.scale2) < 0x1p20f ? m + 8.f / a.scale2 : m;
             l *= al;
 #pragma unroll
             for (int i = 0; i < ND; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[i][r] *= al;
         }
-        const float base = m == -INFINITY ? 0.f : m * a.scale2;   // nothing seen yet: p = 0
+        // fp16 ends at 2^-24: weights below it would count in their sum but not in the product (5000 keys of
+        // 2^-26 beside one of 1: 7.5e-5 of the output).  They, and with them sums and products, are taken 2^7
+        // times as large: with the 2^8 above at most 2^15, inside 65504.  (Past scores of 2^20, where fp32 no
+        // longer holds the exponents to 2^-4, no maximum is kept.)
+        const float base = m == -INFINITY ? 0.f : BF16 ? m * a.scale2 : fmaf(m, a.scale2, -7.f);   // nothing seen yet: p = 0
         u32x4 p[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h)

@@ -45,6 +45,47 @@ def test_prompt_values_that_are_not_finite_in_the_last_row(dev, dt, heads, kv, D
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv,D,lens,past", [
+    (64, 8, 64, [1000], [0]), (64, 8, 128, [1000], [0]),      # 128 queries a block
+    (64, 8, 64, [100], [9000]), (64, 8, 128, [100], [6000]),    # and split
+    (4, 4, 64, [90], [60]), (16, 2, 128, [3], [2000]),        # each wave its own keys; split
+    (64, 8, 128, [2100], [3100])])                            # 256 queries a block
+def test_prompt_many_small_weights_beside_a_great_one(dev, heads, kv, D, lens, past, causal):
+    """fp16: a key of weight 1 and value 0, all others of weight w = e^-18 < 2^-25 and value c: out is
+    n w c / (1 + n w) of the n that a query sees.  A weight is rounded as 2^7 w, a subnormal: half of
+    2^-24 at most, 2^-32 c in all for each of them (the sum of weights is 1 at least)."""
+    n_q, n_k = lens[0], lens[0] + past[0]
+    q = torch.ones(n_q, heads, D, dtype=FP)
+    k, v = torch.zeros(n_k, kv, D, dtype=FP), torch.empty(n_k, kv, D, dtype=FP)
+    k[0] = 144 / D
+    v[:] = (32 + torch.arange(D) * 0.5).to(FP)
+    v[0] = 0
+    assert float((q[0, 0] * k[0, 0]).sum()) == 144
+    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), _i32([0, n_q], dev), _i32([0, n_k], dev), scale=0.125,
+                      causal=causal).cpu().double()
+    n = (torch.arange(n_q) + n_k - n_q if causal else torch.full((n_q,), n_k - 1)).double()[:, None]
+    c, w, h = v[-1, 0].double()[None], math.exp(-18.0), ref.half_step(FP)
+    want = n * w * c / (1 + n * w)
+    tol = h * want + 2.0 ** -25 + n * c * (2.0 ** -32 + w * (2 * 18 * (D + 8) * 2.0 ** -24 + n_k * 2.0 ** -24))
+    assert ((got - want[:, None]).abs() <= tol[:, None]).all()
+
+
+@pytest.mark.parametrize("D,heads", [(64, 4), (128, 4), (64, 64), (128, 64)])
+@pytest.mark.parametrize("top", [16, 19, 20, 21, 24, 26])
+def test_prompt_scores_of_many_millions(dev, D, heads, top):
+    """fp16: scores that rise to 2^top powers of two, 2^(top - 9) a key: a query gets the value of its
+    last key, through one rounding of its weight and one of the output."""
+    n = 512
+    _, _, v, cu, _ = _prompt_case([n], heads, 2, D, FP, 71)
+    q = torch.ones(n, heads, D, dtype=FP)
+    k = torch.arange(1, n + 1).to(FP)[:, None, None].expand(n, 2, D).contiguous()
+    scale = 2.0 ** (top - 9) * math.log(2.0) / D
+    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), scale=scale).cpu().double()
+    want = v.double().repeat_interleave(heads // 2, 1)
+    assert ((got - want).abs() <= 2.01 * ref.half_step(FP) * want.abs() + 2.0 ** -24).all()
+
+
 # --- eviction ------------------------------------------------------------------------------------------
 def _cut(x, heads, kv):
     return x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
