@@ -82,10 +82,21 @@ __device__ __forceinline__ double rope_turns(const RopeTable &t, int i) {
     return f;
 }
 
+// A prompt's rows and single tokens are rotated in different kernels and have to give the same bits: the
+// two functions below say where products and sums are rounded once, and contract nothing by themselves.
+
 // cos and sin of pos * turns (in turns), reduced to half a turn in 64 bits.
 __device__ __forceinline__ void rope_cs(int pos, double turns, float &c, float &s) {
-    const double a = pos * turns;
-    sincospif(2.f * static_cast<float>(a - rint(a)), &s, &c);
+#pragma clang fp contract(off)
+    const double p = pos;
+    sincospif(2.f * static_cast<float>(fma(p, turns, -rint(p * turns))), &s, &c);
+}
+
+// The pair (x1, x2) turned.
+__device__ __forceinline__ void rope_turn(float x1, float x2, float c, float s, float &y1, float &y2) {
+#pragma clang fp contract(off)
+    y1 = fmaf(x1, c, -(x2 * s));
+    y2 = fmaf(x1, s, x2 * c);
 }
 
 }  // namespace hxq

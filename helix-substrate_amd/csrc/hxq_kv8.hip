@@ -176,8 +176,9 @@ __global__ __launch_bounds__(kThr) void kv8_append_kernel(const AppendArgs a) {
         load8<DT>(p, at + i0 + HALF, x2);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            y1[j] = rope ? x1[j] * c[j] - x2[j] * s[j] : x1[j];
-            y2[j] = rope ? x2[j] * c[j] + x1[j] * s[j] : x2[j];
+            y1[j] = x1[j];
+            y2[j] = x2[j];
+            if (rope) rope_turn(x1[j], x2[j], c[j], s[j], y1[j], y2[j]);
         }
         lo = pack8<BF16>(y1);
         hi = pack8<BF16>(y2);
@@ -445,10 +446,7 @@ __global__ __launch_bounds__(kDThr, 1) void kv8_decode_kernel(const DecodeArgs a
         const int e = threadIdx.x + i * kDThr, h = e / HALF, d = e % HALF;
         if (h > kHT) break;
         float y1 = x1[i], y2 = x2[i];
-        if (rope) {
-            y1 = x1[i] * cs[d] - x2[i] * sn[d];
-            y2 = x2[i] * cs[d] + x1[i] * sn[d];
-        }
+        if (rope) rope_turn(x1[i], x2[i], cs[d], sn[d], y1, y2);
         if (h == kHT) {
             const uint32_t w = pack16<BF16>(y1, y2);
             kn[d] = static_cast<uint16_t>(w);

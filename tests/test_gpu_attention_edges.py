@@ -8,7 +8,8 @@ import torch
 
 import attention_ref as ref
 from helix_substrate.attention import BLOCK, HelixKV8Cache, attn_prompt, kv8_evict
-from test_gpu_attention import (BF, F32, FP, _check_attend, _cpu, _gen, _i32, _prompt_case, _rows)
+from test_gpu_attention import (BF, F32, FP, _check_attend, _cpu, _gen, _i32, _prompt_case, _rows,
+                                _same_bits)
 
 pytestmark = pytest.mark.gpu
 
@@ -169,3 +170,33 @@ def test_read_next_to_the_end_of_fp16(dev):
     for got in cache.read(0, BLOCK):
         assert got[0, 0, :5].tolist() == [65504.0, -65504.0, 65504.0, -65504.0, 61440.0]
         assert got[1, 0, 0].isnan() and (got[2:] == 0).all()
+
+
+@pytest.mark.parametrize("dt", [F32, BF, FP])
+@pytest.mark.parametrize("cdt", [BF, FP])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("table", [True, False])
+def test_the_same_bits_however_tokens_come(dev, dt, cdt, D, table):
+    """One prompt, pieces of it, tokens one by one, and pieces with tokens between them: rows, blocks and
+    tails of every kernel instance, at positions that turn a pair many times, with a table and without."""
+    heads, kv, n, at = 4, 2, 200, 70_000
+    x = _rows(n, heads, kv, D, dt, 81).to(dev)
+    new = lambda: HelixKV8Cache.empty(1, kv, D, 256, dtype=cdt, device=dev, table=table)
+    put = lambda c, a, b: c.append(*_cut(x[a:b], heads, kv), _i32([a], dev), _i32([0, b - a], dev),
+                                   pos=_i32([at + a], dev), theta=1e4)
+    one = lambda c, a: c.attend(*_cut(x[a:a + 1], heads, kv), _i32([a], dev), pos=_i32([at + a], dev), theta=1e4)
+    whole, pieces, tokens, mixed = (new() for _ in range(4))
+    rows = put(whole, 0, n)
+    cut = [put(pieces, a, b) for a, b in ((0, 1), (1, 63), (63, 128), (128, 131), (131, n))]
+    for i, t in enumerate(rows):
+        assert torch.equal(torch.cat([c[i] for c in cut]), t)
+    for t in range(n):
+        one(tokens, t)
+    put(mixed, 0, 60)
+    for t in range(60, 66):
+        one(mixed, t)
+    put(mixed, 66, 190)
+    for t in range(190, n):
+        one(mixed, t)
+    for c in (pieces, tokens, mixed):
+        _same_bits(c, whole, [n])
