@@ -7,9 +7,11 @@ import pytest
 import torch
 
 import attention_ref as ref
-from helix_substrate.attention import BLOCK, HelixKV8Cache, attn_prompt, kv8_evict
-from test_gpu_attention import (BF, F32, FP, _check_attend, _cpu, _gen, _i32, _prompt_case, _rows,
-                                _same_bits)
+from helix_substrate import _hxq
+from helix_substrate.attention import BLOCK, HelixKV8Cache, attn_prompt, kv8_evict, rope_rows
+from test_gpu_attention import (BF, F32, FP, _check_attend, _check_prompt, _cpu, _ends, _filled, _gen,
+                                _i32, _prompt_case, _rows, _same_bits)
+from test_gpu_attention import test_append as check_append
 
 pytestmark = pytest.mark.gpu
 
@@ -200,3 +202,79 @@ def test_the_same_bits_however_tokens_come(dev, dt, cdt, D, table):
         one(mixed, t)
     for c in (pieces, tokens, mixed):
         _same_bits(c, whole, [n])
+
+
+# --- forms that nothing else reaches -----------------------------------------------------------------------
+@pytest.mark.parametrize("dt,cdt", [(BF, FP), (FP, BF)])
+@pytest.mark.parametrize("heads,kv,D", [(16, 2, 128), (5, 5, 64)])
+def test_append_of_the_other_16_bit_type(dev, dt, cdt, heads, kv, D):
+    check_append(dev, dt, cdt, heads, kv, D, [100, 5, 0], [28, 300, 0])
+
+
+@pytest.mark.parametrize("cdt,dt,odt", [(BF, F32, BF), (FP, F32, F32)])
+@pytest.mark.parametrize("heads,kv,D", [(16, 2, 128), (20, 2, 64)])
+def test_attend_without_a_table(dev, cdt, dt, odt, heads, kv, D):
+    past = [0, 63, 300]
+    cache = _filled(3, kv, D, cdt, past, 6, dev, 91, table=False)
+    assert cache.blocks is None
+    x = _rows(3, heads, kv, D, dt, 92)
+    before = _cpu(cache)
+    got, weight = cache.attend(*_cut(x.to(dev), heads, kv), _i32(past, dev), theta=1e6,
+                               weight_out=cache.new_weight(), out_dtype=odt)
+    now = _cpu(cache)
+    for b, p in enumerate(past):
+        before.k_tail[b, :, p % BLOCK] = now.k_tail[b, :, p % BLOCK]
+        before.v_tail[b, :, :, p % BLOCK] = now.v_tail[b, :, :, p % BLOCK]
+    _check_attend(before, x, heads, past, past, got, weight, 1e6, odt)
+    at = 63 // BLOCK
+    for name in "kv":      # the second sequence's token ended its first block, which lies in its place
+        want, sc = ref.to8(getattr(now, name + "_tail")[1].reshape(kv, -1))
+        assert torch.equal(getattr(now, name)[1, :, at].reshape(kv, -1).float(), want.float())
+        assert torch.equal(getattr(now, name + "_scale")[1, :, at], sc)
+
+
+@pytest.mark.parametrize("dt", [F32, BF, FP])
+@pytest.mark.parametrize("out", [BF, FP])
+@pytest.mark.parametrize("heads,kv,D,theta", [(16, 2, 128, 1e6), (5, 5, 64, 1e4), (4, 1, 64, 0.0)])
+def test_rope_rows(dev, dt, out, heads, kv, D, theta):
+    """Rows rotated without a cache: values, positions far out, given outputs, rows that are left alone."""
+    lens, pos = [70, 0, 5, 64], [0, 9, -1, 131_072]
+    x = _rows(sum(lens) + 3, heads, kv, D, dt, 95)
+    cu = _ends(lens)
+    q, k, v = rope_rows(*_cut(x.to(dev), heads, kv), cu.to(dev), _i32(pos, dev), theta, dtype=out)
+    outs = tuple(torch.full_like(t, 7.0) for t in (q, k, v))
+    same = rope_rows(*_cut(x.to(dev), heads, kv), cu.to(dev), _i32(pos, dev), theta, dtype=out, outs=outs)
+    h, tiny = ref.half_step(out), torch.finfo(out).smallest_normal * ref.half_step(out)
+    for got, mine, src in zip((q, k, v), same, _cut(x, heads, kv)):
+        assert got.dtype == out
+        for s in range(len(lens)):
+            r = slice(int(cu[s]), int(cu[s + 1]))
+            if pos[s] < 0:
+                assert (mine[r] == 7).all()
+                continue
+            want, off = (src[r].double(), 0.0) if got is v else ref.rotate(
+                src[r], pos[s] + torch.arange(lens[s]), theta)
+            assert ((got[r].cpu().double() - want).abs() <= h * want.abs() + 1.01 * off + tiny).all()
+            assert torch.equal(got[r], mine[r])
+        assert (mine[int(cu[-1]):] == 7).all()
+
+
+def _splits(lens, past, heads, D, dev):
+    """Into how many parts a prompt call cuts the keys: from its workspace."""
+    n = sum(lens)
+    return max(1, _hxq._prompt_workspace(n, n + sum(past), len(lens), heads, D, dev.index or 0) // (n * heads * (D * 4 + 8)))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dt,heads,kv,D,lens,past,splits", [
+    (FP, 16, 4, 64, [512, 130, 1, 400, 257, 512], [7000, 6500, 7100, 0, 5000, 7000], 2),   # by die, tiles of 128
+    (BF, 28, 4, 128, [300, 129, 40], [3000, 2500, 900], 3),
+    (BF, 64, 8, 128, [100, 64], [6000, 5000], 4),
+    (FP, 4, 4, 64, [40, 3], [900, 1200], 3)])                                            # each wave its own keys
+def test_prompt_splits_of_ragged_batches(dev, dt, heads, kv, D, lens, past, splits, causal):
+    """Several sequences of several tiles with their keys in parts, on 256 compute units."""
+    if torch.cuda.get_device_properties(dev).multi_processor_count == 256:
+        assert _splits(lens, past, heads, D, dev) == splits
+    q, k, v, cu, cu_k = _prompt_case(lens, heads, kv, D, dt, 97, past)
+    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu_k.to(dev), causal=causal)
+    _check_prompt(got, q, k, v, cu, cu_k, causal=causal)
