@@ -67,6 +67,7 @@ class HxqKv8(ctypes.Structure):
         ("blocks", P), ("dtype", I32), ("batch", I32), ("n_kv_heads", I32), ("head_dim", I32),
         ("n_blocks", I32),
     ]
+    device = None   # of the tensors; None: no cache, rows only
 
 
 class HxqDecoder(ctypes.Structure):
@@ -927,8 +928,10 @@ def kv8_desc(k, v, k_scale, v_scale, k_tail, v_tail, blocks):
             or v_tail.shape != (batch, n_kv, D, block)
             or (blocks is not None and blocks.shape != each)):
         raise ValueError("cache shapes do not fit together")
-    return HxqKv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+    desc = HxqKv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                   k_tail.data_ptr(), v_tail.data_ptr(), _ptr(blocks), dt, batch, n_kv, D, n_blocks)
+    desc.device = dev
+    return desc
 
 
 def kv8_append(q, k, v, cu_rows, cached, pos, theta, desc, outs):
@@ -946,6 +949,8 @@ def kv8_append(q, k, v, cu_rows, cached, pos, theta, desc, outs):
         raise ValueError("q must be [rows, heads, D], k and v [rows, kv heads, D] of the cache")
     if dt != v.dtype or (q is not None and q.dtype != dt):
         raise RuntimeError("q, k and v must have one dtype")
+    if desc.device is not None and desc.device != dev:
+        raise RuntimeError(f"the cache is on cuda:{desc.device}, not on cuda:{dev}")
     batch, i32 = desc.batch, torch.int32
     if not (cu_rows.dtype == cached.dtype == i32 and (pos is None or pos.dtype == i32)):
         raise RuntimeError("cu_rows, cached and pos must be int32")
@@ -984,6 +989,8 @@ def kv8_attn_decode(q, k, v, cached, pos, theta, scale, desc, weight, weight_out
         _why(dev, (("q", q), ("k", k), ("v", v)),
              (("cached", cached), ("pos", pos), ("weight", weight), ("weight_out", weight_out),
               ("out", out)))
+    if desc.device != dev:
+        raise RuntimeError(f"the cache is on cuda:{desc.device}, not on cuda:{dev}")
     batch, heads, D = qs
     n_kv, n_blocks = ks[1], desc.n_blocks
     if (batch != desc.batch or D != desc.head_dim or n_kv != desc.n_kv_heads or v.shape != ks

@@ -278,3 +278,16 @@ def test_prompt_splits_of_ragged_batches(dev, dt, heads, kv, D, lens, past, spli
     q, k, v, cu, cu_k = _prompt_case(lens, heads, kv, D, dt, 97, past)
     got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu_k.to(dev), causal=causal)
     _check_prompt(got, q, k, v, cu, cu_k, causal=causal)
+
+
+def test_a_cache_on_another_device_is_refused(dev):
+    """Rows on one device, the cache on another: its addresses mean nothing there."""
+    heads, kv, D = 4, 2, 64
+    cache = HelixKV8Cache.empty(1, kv, D, 128, device=dev)
+    x, n = _rows(1, heads, kv, D, BF, 99).to(dev), _i32([0], dev)
+    assert cache._desc.device == x.get_device()
+    cache._desc.device += 1      # as of a cache there
+    with pytest.raises(RuntimeError, match="cache is on"):
+        cache.attend(*_cut(x, heads, kv), n)
+    with pytest.raises(RuntimeError, match="cache is on"):
+        cache.append(*_cut(x, heads, kv), n, _i32([0, 1], dev))
