@@ -291,3 +291,46 @@ def test_a_cache_on_another_device_is_refused(dev):
         cache.attend(*_cut(x, heads, kv), n)
     with pytest.raises(RuntimeError, match="cache is on"):
         cache.append(*_cut(x, heads, kv), n, _i32([0, 1], dev))
+
+
+def test_a_prompt_a_token_and_an_eviction_captured(dev):
+    """The whole run in one graph, replayed over a cache that each replay cuts again, with eager work
+    between; every replay equals the eager run."""
+    heads, kv, D, n, theta = 8, 2, 128, 150, 1e6
+    xs = [_rows(n + 1, heads, kv, D, BF, 110 + i).to(dev) for i in range(4)]
+    cu = _i32([0, n], dev)
+
+    def step(cache, x, cached, pos, w):
+        q, k, v = cache.append(*_cut(x[:n], heads, kv), cached, cu, pos=pos, theta=theta)
+        o = attn_prompt(q, k, v, cu)
+        cached += n
+        pos += n
+        one, _ = cache.attend(*_cut(x[n:], heads, kv), cached, pos=pos, theta=theta, weight=w, weight_out=w)
+        cached += 1
+        pos += 1
+        cached.copy_(cache.evict(w, cached, keep=3, sink=1, recent=1))
+        return o, one
+
+    def fresh():
+        cache = HelixKV8Cache.empty(1, kv, D, 512, device=dev)
+        return cache, _i32([0], dev), _i32([0], dev), cache.new_weight()
+
+    cache, cached, pos, w = fresh()
+    want = []
+    for x in xs:
+        o, one = step(cache, x, cached, pos, w)
+        want.append([t.clone() for t in (o, one, cached, pos, w, cache.blocks, cache.k.view(torch.uint8), cache.v_scale)])
+    assert int(want[-1][2]) == 192 + (4 * (n + 1)) % 64
+    cache, cached, pos, w = fresh()
+    x = xs[0].clone()
+    s, g = torch.cuda.Stream(device=dev), torch.cuda.CUDAGraph()
+    s.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+        o, one = step(cache, x, cached, pos, w)
+    torch.cuda.current_stream(dev).wait_stream(s)
+    for i, right in enumerate(want):
+        x.copy_(xs[i])
+        g.replay()
+        torch.randn(1 << 20, device=dev).sum().item()
+        for a, b in zip((o, one, cached, pos, w, cache.blocks, cache.k.view(torch.uint8), cache.v_scale), right):
+            assert torch.equal(a, b), i
