@@ -1026,6 +1026,8 @@ def _kv8_workspace(batch, heads, n_kv, D, n_blocks, weights, device):
 
 def kv8_evict(weight, blocks, cached, keep, sink, recent):
     """Choose the blocks that stay (hxq_kv8_evict).  Returns new blocks, weight, cached."""
+    if keep >= 1 << 31 or sink >= 1 << 31 or recent >= 1 << 31:   # ctypes would wrap them
+        raise ValueError("keep, sink and recent must be less than 2^31")
     dev, shape, i32 = weight.get_device(), weight.shape, torch.int32
     if not (dev >= 0 and _flat(weight, dev) and _flat(blocks, dev) and _flat(cached, dev)):
         _why(dev, (), (("weight", weight), ("blocks", blocks), ("cached", cached)))
