@@ -199,11 +199,12 @@ __device__ __forceinline__ void store_rows(const f32x16 (&o)[ND], float inv, uin
 // the chip, where the chain of a block's steps is the time.
 // SPLIT: blockIdx.y takes a part of the keys and leaves its sums for attn_join_kernel.
 //
-// Bound by the issue of MFMA, softmax and LDS reads together (of 1070 us the arithmetic of the softmax
-// is 14 %, the global loads 13 %, the LDS reads 10 %; the matrix pipe is busy half the time).  P in the
-// operands' 16 bits: half a step of each weight, of the size of the output's own rounding.  Measured:
-// 16 heads over 2, 16384 tokens 990 us (1.11 PFLOP/s); 28 over 4, twelve sequences of 371 to 2048 223;
-// fp16 at head_dim 64, six pieces over 7000 keys 103; 211 tokens 8.2 (KW).
+// Bound by the issue of MFMA, softmax and LDS reads together: the matrix pipe is busy 54 % of the cycles,
+// LDS 34 %, without bank conflicts.  P in the operands' 16 bits: half a step of each weight, of the size of
+// the output's own rounding.  Measured: 16 heads over 2, 16384 tokens 1007 us (1.09 PFLOP/s); 28 over 4,
+// twelve sequences of 371 to 2048 226; fp16 at head_dim 64, six pieces over 7000 keys 98 and 6 of the join;
+// 211 tokens 8.9 (KW).  Pairs of times above and in the rules below were measured side by side; cards differ
+// by 3 %.
 template <int NW, bool BF16, int D, bool CAUSAL, bool SPLIT, bool KW = false>
 __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(const PromptArgs a) {
     constexpr int THR = KW ? 64 : 64 * NW, BM = KW ? 32 : 32 * NW, NB = KW || D == 64 ? 1 : 2;

@@ -55,8 +55,8 @@ def kv8_evict(weight, blocks, cached, keep, sink=0, recent=0):
 
 class HelixKV8Cache:
     """Keys and values of `batch` sequences in blocks of 64 tokens, e4m3 with a power-of-two scale
-    per block and kv head; the unfinished block of each in 16 bits.  2.03 bytes per token, head and
-    dimension pair against 4 of a bf16 cache.
+    per block and kv head; the unfinished block of each in 16 bits.  Per kv head: 2 D bytes a token
+    (4 D in a bf16 cache), 12 a block and 256 D a sequence.
 
     k, v: float8_e4m3fn [batch, n_kv, n_blocks, 64, D] and [batch, n_kv, n_blocks, D, 64];
     k_scale, v_scale: fp32 [batch, n_kv, n_blocks]; k_tail, v_tail: bf16 or fp16 [batch, n_kv, 64, D]

@@ -542,7 +542,8 @@ int hxq_argmax(const float *logits, int64_t n, int32_t *out_id, int32_t *pos,
  * prompt that continues cached tokens passes them as its first keys.  A query that sees no key
  * gives zeros; one whose scores are all -inf gives NaN.  Keys that a query does not see have no
  * influence, whatever they hold.  dtype (q, k, v, out): HXQ_BF16 or HXQ_F16; scores, softmax and sums
- * are fp32, the softmax weights are rounded to dtype before the product with v.  Rows of out that
+ * are fp32, the softmax weights are rounded to dtype before the product with v; scores have to stay
+ * below 2^26 (beyond, the greatest weight may leave dtype's range, and out be NaN).  Rows of out that
  * belong to no sequence are left as they were; offsets are clamped to [0, rows_q] and [0, rows_k].
  * scale: 2^-100 to 2^100.  Row strides of k and v: 0 to 2^24 - 1 elements.  out may be q, and must
  * not overlap k or v.  workspace: device scratch of hxq_attn_prompt_workspace_bytes(...) bytes (0 in
