@@ -334,3 +334,97 @@ def test_a_prompt_a_token_and_an_eviction_captured(dev):
         torch.randn(1 << 20, device=dev).sum().item()
         for a, b in zip((o, one, cached, pos, w, cache.blocks, cache.k.view(torch.uint8), cache.v_scale), right):
             assert torch.equal(a, b), i
+
+
+# --- many sequences, wide groups, extreme arguments --------------------------------------------------------
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dt,heads,kv,D,long", [
+    (BF, 1, 1, 128, False), (FP, 2, 1, 64, False),     # each wave its own keys; split and not
+    (BF, 4, 2, 128, True), (FP, 4, 4, 64, True)])      # sequences of several tiles
+def test_prompt_of_more_sequences_than_lanes(dev, dt, heads, kv, D, long, causal):
+    """The tiles of 150 sequences, some without queries, some without keys, found in rounds of 64."""
+    n = 150
+    lens = [(37 * i) % 301 if long and i % 3 == 0 else (7 * i) % 6 for i in range(n)]
+    past = [(53 * i) % 701 if i % 4 else -lens[i] for i in range(n)]
+    q, k, v, cu, cu_k = _prompt_case(lens, heads, kv, D, dt, 121, past)
+    got = attn_prompt(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu_k.to(dev), causal=causal)
+    _check_prompt(got, q, k, v, cu, cu_k, causal=causal)
+
+
+@pytest.mark.parametrize("heads", [4, 64])
+def test_prompt_without_any_key(dev, heads):
+    q, _, _, cu, _ = _prompt_case([70, 3], heads, 2, 64, BF, 122)
+    none = torch.empty(0, 2, 64, dtype=BF, device=dev)
+    got = attn_prompt(q.to(dev), none, none, cu.to(dev), torch.zeros(3, dtype=torch.int32, device=dev))
+    assert (got == 0).all()
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("heads", [4, 64])
+def test_prompt_scale_at_its_ends(dev, dt, heads):
+    """2^-100: the mean of what a query sees.  2^100 over products of 2^-100: as 1 over products of 1."""
+    q, k, v, cu, _ = _prompt_case([200], heads, 2, 128, dt, 123)
+    a = [t.to(dev) for t in (q, k, v, cu)]
+    got = attn_prompt(*a, scale=2.0 ** -100)
+    _check_prompt(got, q * 0, k, v, cu, cu)
+    if dt == BF:
+        small = attn_prompt(a[0] * 2.0 ** -50, a[1] * 2.0 ** -50, *a[2:], scale=2.0 ** 100)
+        assert torch.equal(small, attn_prompt(*a, scale=1.0))
+
+
+def test_append_and_attend_of_more_sequences_than_lanes(dev):
+    """150 sequences, some skipped, some without rows: each as in a call of its own."""
+    heads, kv, D, n, theta = 4, 2, 64, 150, 1e4
+    lens = [(29 * i) % 140 if i % 3 else 0 for i in range(n)]
+    cached = [-1 if i % 11 == 5 else (17 * i) % 100 for i in range(n)]
+    cu, x = _ends(lens), _rows(sum(lens), heads, kv, D, BF, 131).to(dev)
+    first = _rows(100, heads, kv, D, BF, 132).to(dev)
+    t = _rows(n, heads, kv, D, F32, 133).to(dev)
+    cache = HelixKV8Cache.empty(n, kv, D, 256, device=dev)
+    fill = _ends([max(c, 0) for c in cached])
+    rows = torch.cat([first[:max(c, 0)] for c in cached])
+    cache.append(*_cut(rows, heads, kv), _i32([0] * n, dev), fill.to(dev), theta=theta)
+    outs = tuple(torch.full((sum(lens), h, D), 7.0, dtype=BF, device=dev) for h in (heads, kv, kv))
+    cache.append(*_cut(x, heads, kv), _i32(cached, dev), cu.to(dev), theta=theta, outs=outs)
+    now = [c if c < 0 else c + m for c, m in zip(cached, lens)]
+    w = torch.full((n, kv, 4), 3.0, device=dev)
+    out = torch.full((n, heads, D), 5.0, device=dev)
+    cache.attend(*_cut(t, heads, kv), _i32(now, dev), theta=theta, weight_out=w, out=out)
+    for i in range(0, n):
+        r = slice(int(cu[i]), int(cu[i + 1]))
+        if cached[i] < 0:
+            assert all((o[r] == 7).all() for o in outs) and (out[i] == 5).all() and (w[i] == 3).all()
+            assert (cache.k[i].view(torch.uint8) == 0).all() and (cache.k_tail[i] == 0).all()
+            continue
+        if i % 7:
+            continue
+        one = HelixKV8Cache.empty(1, kv, D, 256, device=dev)
+        one.append(*_cut(first[:cached[i]], heads, kv), _i32([0], dev), _i32([0, cached[i]], dev), theta=theta)
+        mine = one.append(*_cut(x[r], heads, kv), _i32([cached[i]], dev), _i32([0, lens[i]], dev), theta=theta)
+        for a, b in zip(mine, outs):
+            assert torch.equal(a, b[r])
+        o, ww = one.attend(*_cut(t[i:i + 1], heads, kv), _i32([now[i]], dev), theta=theta,
+                           weight_out=one.new_weight(), out_dtype=F32)
+        held = now[i] + 1
+        assert torch.equal(cache.k[i].view(torch.uint8), one.k[0].view(torch.uint8))
+        assert torch.equal(cache.v_tail[i][..., :held % BLOCK], one.v_tail[0][..., :held % BLOCK])
+        assert torch.equal(out[i], o[0]) and torch.equal(w[i], ww[0])      # one split in both
+
+
+@pytest.mark.parametrize("cdt,dt,odt", [(FP, F32, F32), (BF, FP, F32)])
+@pytest.mark.parametrize("heads,kv,D", [(20, 2, 64), (16, 1, 128), (7, 7, 64), (9, 1, 64)])
+def test_attend_long_of_other_groups(dev, cdt, dt, odt, heads, kv, D):
+    """More than eight query heads a kv head over many splits, a token that ends its block among them."""
+    past = [6000, 64 * 90 + 63, 0, 64 * 40]
+    cache = _filled(4, kv, D, cdt, past, 96, dev, 141)
+    x = _rows(4, heads, kv, D, dt, 142)
+    x[:, heads:heads + kv] *= 0.3
+    before = _cpu(cache)
+    w = torch.full((4, kv, 96), 0.25, device=dev)
+    got, weight = cache.attend(*_cut(x.to(dev), heads, kv), _i32(past, dev), theta=1e6, weight=w, weight_out=w,
+                               out_dtype=odt)
+    now = _cpu(cache)
+    for b, p in enumerate(past):
+        before.k_tail[b, :, p % BLOCK] = now.k_tail[b, :, p % BLOCK]
+        before.v_tail[b, :, :, p % BLOCK] = now.v_tail[b, :, :, p % BLOCK]
+    _check_attend(before, x, heads, past, past, got, weight, 1e6, odt, w0=0.25)
